@@ -26,11 +26,13 @@ enum DataType : int32_t {  // prebuild/defs.hpp:8-18
   DT_FLOAT32,
   DT_UINT64,
   DT_INT64,
+  DT_FLOAT8_E4M3 = LLMHIP_DT_FLOAT8_E4M3,  // of a cache in pages only; not one of the reference's
 };
 
 // Bytes of `size` elements (prebuild/defs.hpp:20-41); (size_t)-1 for an unknown type.
 inline size_t SizeOfTensor(size_t size, DataType dt) {
   static const int width[] = {1, 1, 4, 4, 2, 2, 4, 8, 8};
+  if (dt == DT_FLOAT8_E4M3) return size;
   if (dt < DT_UINT8 || dt > DT_INT64) return static_cast<size_t>(-1);
   return size * static_cast<size_t>(width[dt]);
 }
@@ -150,6 +152,36 @@ inline void hip_decode_step_gqa_layer(void *output_dev, void *k_cache_dev, void 
   CHECK_LLMHIP(llmhip_decode_step_gqa(output_dev, k_cache_dev, v_cache_dev, freqs_cis_dev, input_q_dev,
                                       input_k_dev, input_v_dev, pos, group_size, kv_head_num, head_dim,
                                       is_neox_style ? 1 : 0, dt, stream));
+}
+
+// A KV cache in pages of 16 or 8 bits and a batch of sequences over it (llmhip.h); no counterparts in the reference header.
+inline void hip_paged_rope_kv_append_layer(void *output_q_dev, void *k_pages_dev, void *v_pages_dev, const int *page_table_dev,
+                                           const int *q_starts_dev, const int *kv_lens_dev, void *freqs_cis_dev, void *input_q_dev,
+                                           void *input_k_dev, void *input_v_dev, int tokens, int batch, int pages_per_seq, int num_pages,
+                                           int page_size, int64_t page_stride, int table_rows, int n_heads, int n_kv_heads,
+                                           int head_dim, bool is_neox_style, DataType cache_dt, DataType dt, gpuStream_t &stream) {
+  CHECK_LLMHIP(llmhip_paged_rope_kv_append(output_q_dev, k_pages_dev, v_pages_dev, page_table_dev, q_starts_dev, kv_lens_dev, freqs_cis_dev,
+                                           input_q_dev, input_k_dev, input_v_dev, tokens, batch, pages_per_seq, num_pages, page_size,
+                                           page_stride, table_rows, n_heads, n_kv_heads, head_dim, is_neox_style ? 1 : 0, cache_dt, dt,
+                                           stream));
+}
+
+inline void hip_paged_flash_attn_gqa_layer(void *output_dev, void *q_dev, void *k_pages_dev, void *v_pages_dev, const int *page_table_dev,
+                                           const int *q_starts_dev, const int *kv_lens_dev, void *workspace_dev, size_t workspace_bytes,
+                                           int tokens, int batch, int max_q_len, int max_kv_len, int pages_per_seq, int num_pages,
+                                           int page_size, int64_t page_stride, int window, int sinks, int group_size, int kv_head_num,
+                                           int head_dim, DataType cache_dt, DataType dt, gpuStream_t &stream) {
+  CHECK_LLMHIP(llmhip_paged_flash_attn_gqa(output_dev, q_dev, k_pages_dev, v_pages_dev, page_table_dev, q_starts_dev, kv_lens_dev, workspace_dev,
+                                           workspace_bytes, tokens, batch, max_q_len, max_kv_len, pages_per_seq, num_pages, page_size,
+                                           page_stride, window, sinks, group_size, kv_head_num, head_dim, cache_dt, dt, stream));
+}
+
+inline void hip_paged_kv_read_layer(void *output_k_dev, void *output_v_dev, void *k_pages_dev, void *v_pages_dev, const int *page_table_dev,
+                                    const int *q_starts_dev, const int *kv_lens_dev, int tokens, int batch, int pages_per_seq, int num_pages,
+                                    int page_size, int64_t page_stride, int kv_head_num, int head_dim, DataType cache_dt, DataType dt,
+                                    gpuStream_t &stream) {
+  CHECK_LLMHIP(llmhip_paged_kv_read(output_k_dev, output_v_dev, k_pages_dev, v_pages_dev, page_table_dev, q_starts_dev, kv_lens_dev, tokens, batch,
+                                    pages_per_seq, num_pages, page_size, page_stride, kv_head_num, head_dim, cache_dt, dt, stream));
 }
 
 }  // namespace llm_simple_amd

@@ -27,6 +27,7 @@ extern "C" {
 
 #define LLMHIP_DT_FLOAT16 4  /* prebuild/defs.hpp:13 */
 #define LLMHIP_DT_BFLOAT16 5 /* prebuild/defs.hpp:14 */
+#define LLMHIP_DT_FLOAT8_E4M3 16 /* of a cache in pages only; not one of the reference's types */
 
 #define LLMHIP_OK 0
 #define LLMHIP_ERR_INVALID_ARG (-1)   /* null or misaligned pointer, non-positive size, bad dtype */
@@ -183,6 +184,62 @@ int llmhip_rope_kv_append(void *out_q, void *k_cache, void *v_cache, const void 
                           const void *in_q, const void *in_k, const void *in_v,
                           int start_pos, int cur_size, int n_heads, int n_kv_heads,
                           int head_dim, int is_neox_style, int dt, void *stream);
+
+/* ------------------------------------------------------------------ */
+/* a KV cache in pages, of 16 or of 8 bits                             */
+/* ------------------------------------------------------------------ */
+/* The reference has one contiguous 16-bit cache of one sequence (src/llama2_layer_npu.cpp:1148-1149) and no counterpart of these.
+ *
+ * Pages.  K and V each have a pool of num_pages pages, page i at k_pages + i * page_stride bytes (page_stride: a multiple of 16, at
+ * least llmhip_paged_page_bytes; one allocation may hold both pools, page by page).  A page holds [kv_head_num][page_size] rows of
+ * head_dim elements of cache_dt; page_size is a multiple of 16, up to 1024.  cache_dt is dt, or LLMHIP_DT_FLOAT8_E4M3: then a row is
+ * 128 e4m3 values times a power of two, 2^(byte - 127), and a page ends with the bytes of its rows, [kv_head_num][page_size].  The
+ * byte is the least one, and at least 64, for which the row's largest magnitude is within 448 * 2^(byte - 127).  (Magnitudes above 61440 in fp16 and
+ * 1.875 * 2^127 in bf16 count as that; an infinity is stored as NaN and does not count in the byte.)
+ * Pools together may be larger than 4 GiB; pages_per_seq * page_size is at most 2^30.
+ *
+ * Batch.  All int32, aligned to 4 bytes, in device memory, read when the work runs (a captured graph may be replayed with others):
+ *   page_table [batch][pages_per_seq]   pages of a sequence's rows, in order.  A number outside of [0, num_pages) is a page that is
+ *                                       not there: nobody sees its keys, and nothing is written for it.
+ *   q_starts [batch + 1]                sequence b's new tokens are rows q_starts[b] .. q_starts[b + 1] of the dense tensors, which
+ *                                       have `tokens` rows; none, one or many.  Rows that are no sequence's are neither read nor written.
+ *   kv_lens [batch]                     rows of the sequence with the new tokens: token t of sequence b is at position
+ *                                       kv_lens[b] - q_starts[b + 1] + t, the last one at kv_lens[b] - 1.
+ * A sequence whose rows are not all within [0, tokens), or whose length is not within [0, pages_per_seq * page_size], is passed over.
+ * No two sequences may write one page, nor have one row.  dense tensors: [tokens][heads][head_dim] of dt. */
+
+/* Bytes of a page of K, or of V; 0 for sizes that the calls below refuse. */
+size_t llmhip_paged_page_bytes(int page_size, int kv_head_num, int head_dim, int cache_dt);
+
+/* llmhip_rope_kv_append for a batch and pages: out_q = rope(in_q), and the pages' rows of the new tokens' positions become rope(in_k) and
+ * in_v, in 8 bits if the cache is.  (8 bits are taken of the row as it would be in a 16-bit cache.)  freq_cis has table_rows rows; a
+ * token whose position is not within [0, table_rows) is passed over.  out_q and in_q may be one buffer. */
+int llmhip_paged_rope_kv_append(void *out_q, void *k_pages, void *v_pages, const int *page_table, const int *q_starts, const int *kv_lens,
+                                const void *freq_cis, const void *in_q, const void *in_k, const void *in_v, int tokens, int batch,
+                                int pages_per_seq, int num_pages, int page_size, int64_t page_stride, int table_rows, int n_heads,
+                                int n_kv_heads, int head_dim, int is_neox_style, int cache_dt, int dt, void *stream);
+
+/* Attention of the new tokens, which llmhip_paged_rope_kv_append has put into the pages before: of one token to a sequence (decode), pieces of
+ * prompts, whole prompts, all of these in one batch.  Query head h reads kv head h / group_size.  A token at position p sees key c if
+ * c <= p and, with window > 0, c > p - window or c < sinks; window <= 0: all keys up to p.  A row that sees no key is zeros.
+ * Keys that a row does not see have no part in it, infinities and NaN included.
+ * max_q_len: no sequence has more new tokens (one that does is passed over).  max_kv_len: no sequence is longer; if one is, the
+ * call is slower and no less right.  They, tokens and batch shape the launch, and may be larger than what is there.
+ * workspace: llmhip_paged_flash_attn_workspace_bytes bytes for the same arguments (0 where no keys are shared among workgroups), of the
+ * caller's, so that the call allocates nothing and may be captured; calls that overlap need one each.  out and q may be one buffer. */
+int llmhip_paged_flash_attn_gqa(void *out, const void *q, const void *k_pages, const void *v_pages, const int *page_table, const int *q_starts,
+                                const int *kv_lens, void *workspace, size_t workspace_bytes, int tokens, int batch, int max_q_len,
+                                int max_kv_len, int pages_per_seq, int num_pages, int page_size, int64_t page_stride, int window,
+                                int sinks, int group_size, int kv_head_num, int head_dim, int cache_dt, int dt, void *stream);
+size_t llmhip_paged_flash_attn_workspace_bytes(int tokens, int batch, int max_q_len, int max_kv_len, int window, int sinks,
+                                               int group_size, int kv_head_num, int head_dim);
+
+/* The way back: out_k, out_v [tokens][kv_head_num][head_dim] of dt = the cached rows at the tokens' positions, what 8 bits stand for exactly
+ * (q_starts decides how many of a sequence's last rows come: all of them where q_starts[b + 1] - q_starts[b] = kv_lens[b]).  Zeros where
+ * there is no such row. */
+int llmhip_paged_kv_read(void *out_k, void *out_v, const void *k_pages, const void *v_pages, const int *page_table, const int *q_starts,
+                         const int *kv_lens, int tokens, int batch, int pages_per_seq, int num_pages, int page_size, int64_t page_stride,
+                         int kv_head_num, int head_dim, int cache_dt, int dt, void *stream);
 
 /* ------------------------------------------------------------------ */
 /* runtime surface used by the device layer                            */

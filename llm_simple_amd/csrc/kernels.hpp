@@ -95,6 +95,18 @@ hipError_t launch_rope_kv_append(void *out_q, void *out_k, void *out_v, const vo
                                  int start_pos, int cur_size, int q_heads, int k_heads,
                                  int k_out_row_offset, int is_neox, int dt, hipStream_t stream);
 
+// A cache in pages (paged.hpp).  Sizes and pointers checked; lengths, starts and page numbers, which are on the device, need not be.
+struct PagedBatch;
+hipError_t launch_paged_append(void *out_q, void *k_pages, void *v_pages, const PagedBatch &batch, const void *freq_cis, const void *in_q,
+                               const void *in_k, const void *in_v, int table_rows, int q_heads, int kv_heads, int is_neox, bool eight,
+                               int dt, hipStream_t stream);
+hipError_t launch_paged_read(void *out_k, void *out_v, const void *k_pages, const void *v_pages, const PagedBatch &batch, int kv_heads,
+                             bool eight, int dt, hipStream_t stream);
+// window 0: all keys.  A workspace of paged_attn_workspace_bytes for the same bounds.
+size_t paged_attn_workspace_bytes(int tokens, int batch, int max_q_len, int max_kv_len, int window, int sinks, int g, int Hkv);
+hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, const void *v_pages, const PagedBatch &batch, void *workspace,
+                             int max_q_len, int max_kv_len, int window, int sinks, int g, int Hkv, bool eight, int dt, hipStream_t stream);
+
 // Projection out[m][n] = round(lhs[m][k] . weight[n][k]^T + bias), bias fp32 [n] or null; n and k multiples
 // of 16.  matmul_skinny: m <= 16, pointers 16-byte aligned.  matmul_tile: the sizes that matmul_tile_takes
 // accepts, pointers 16-byte aligned; with more than one of matmul_tile_pieces' pieces of k a workspace of matmul_pieces_bytes, and not on a

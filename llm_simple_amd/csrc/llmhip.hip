@@ -8,6 +8,7 @@
 #include <mutex>
 
 #include "kernels.hpp"
+#include "paged.hpp"
 #include "stream_scratch.hpp"
 
 using namespace llmhip;
@@ -22,6 +23,7 @@ inline int from_hip(hipError_t e) { return e == hipSuccess ? LLMHIP_OK : (int)e;
 inline bool dtype_ok(int dt) { return dt == LLMHIP_DT_FLOAT16 || dt == LLMHIP_DT_BFLOAT16; }
 // every kernel moves 16-byte pieces: a misaligned base pointer would fault on the device
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 template <typename... P> inline bool all_aligned16(P... ptrs) { return (aligned16(ptrs) && ...); }
 
 // Split-KV scratch for the entry points that mirror the reference signatures
@@ -147,6 +149,35 @@ int attn_common(void *out, const void *q, const void *k, const void *v, int m, i
   if (rc != LLMHIP_OK) return rc;
   return from_hip(launch_flash_prefill(out, q, k, v, m, n, offset, group_size, kv_head_num, dt,
                                        as_stream(stream), ws->ptr, ws->bytes));
+}
+
+// The sizes of a cache in pages and of a batch over it; fills the batch.
+constexpr int kMaxPageSize = 1024, kMaxPagedKeys = 1 << 30;
+bool page_sizes_ok(int page_size, int kv_head_num, int dt) {
+  return page_size >= kPageGroup && page_size <= kMaxPageSize && page_size % kPageGroup == 0 && kv_head_num >= 1 && kv_head_num <= 65535 &&
+         (dtype_ok(dt) || dt == LLMHIP_DT_FLOAT8_E4M3);
+}
+int paged_common(PagedBatch &b, const int *page_table, const int *q_starts, const int *kv_lens, int tokens, int batch, int pages_per_seq,
+                 int num_pages, int page_size, int64_t page_stride, int kv_head_num, int head_dim, int cache_dt, int dt) {
+  if (!page_table || !q_starts || !kv_lens || !aligned4(page_table) || !aligned4(q_starts) || !aligned4(kv_lens)) return LLMHIP_ERR_INVALID_ARG;
+  if (tokens < 1 || batch < 1 || pages_per_seq < 1 || num_pages < 1 || kv_head_num < 1) return LLMHIP_ERR_INVALID_ARG;
+  if (!dtype_ok(dt) || (cache_dt != dt && cache_dt != LLMHIP_DT_FLOAT8_E4M3)) return LLMHIP_ERR_INVALID_ARG;
+  if (page_size < 1) return LLMHIP_ERR_INVALID_ARG;
+  if (head_dim != 128 || !page_sizes_ok(page_size, kv_head_num, cache_dt)) return LLMHIP_ERR_UNSUPPORTED;
+  if ((long long)pages_per_seq * page_size > kMaxPagedKeys) return LLMHIP_ERR_UNSUPPORTED;
+  if (page_stride % 16 != 0 || page_stride < (int64_t)llmhip_paged_page_bytes(page_size, kv_head_num, head_dim, cache_dt))
+    return LLMHIP_ERR_INVALID_ARG;
+  b.page_table = page_table;
+  b.q_starts = q_starts;
+  b.kv_lens = kv_lens;
+  b.batch = batch;
+  b.tokens = tokens;
+  b.pages_per_seq = pages_per_seq;
+  b.num_pages = num_pages;
+  b.keys_max = pages_per_seq * page_size;
+  b.page_size = make_fast_div(page_size);
+  b.page_stride = page_stride;
+  return LLMHIP_OK;
 }
 
 }  // namespace
@@ -323,6 +354,67 @@ int llmhip_rope_kv_append(void *out_q, void *k_cache, void *v_cache, const void 
   return from_hip(launch_rope_kv_append(out_q, k_cache, v_cache, freq_cis, in_q, in_k, in_v,
                                         start_pos, cur_size, n_heads, n_kv_heads, start_pos,
                                         is_neox_style, dt, as_stream(stream)));
+}
+
+/* ---------------- a cache in pages ---------------- */
+
+size_t llmhip_paged_page_bytes(int page_size, int kv_head_num, int head_dim, int cache_dt) {
+  if (head_dim != 128 || !page_sizes_ok(page_size, kv_head_num, cache_dt)) return 0;
+  return (size_t)page_size * kv_head_num * (cache_dt == LLMHIP_DT_FLOAT8_E4M3 ? head_dim + 1 : 2 * head_dim);
+}
+
+int llmhip_paged_rope_kv_append(void *out_q, void *k_pages, void *v_pages, const int *page_table, const int *q_starts, const int *kv_lens,
+                                const void *freq_cis, const void *in_q, const void *in_k, const void *in_v, int tokens, int batch,
+                                int pages_per_seq, int num_pages, int page_size, int64_t page_stride, int table_rows, int n_heads,
+                                int n_kv_heads, int head_dim, int is_neox_style, int cache_dt, int dt, void *stream) {
+  if (!out_q || !k_pages || !v_pages || !freq_cis || !in_q || !in_k || !in_v || !all_aligned16(out_q, k_pages, v_pages, freq_cis, in_q, in_k, in_v))
+    return LLMHIP_ERR_INVALID_ARG;
+  if (table_rows < 1 || n_heads < 1) return LLMHIP_ERR_INVALID_ARG;
+  PagedBatch b;
+  const int rc = paged_common(b, page_table, q_starts, kv_lens, tokens, batch, pages_per_seq, num_pages, page_size, page_stride, n_kv_heads,
+                              head_dim, cache_dt, dt);
+  if (rc != LLMHIP_OK) return rc;
+  if (n_heads > 65535) return LLMHIP_ERR_UNSUPPORTED;
+  return from_hip(launch_paged_append(out_q, k_pages, v_pages, b, freq_cis, in_q, in_k, in_v, table_rows, n_heads, n_kv_heads, is_neox_style,
+                                      cache_dt == LLMHIP_DT_FLOAT8_E4M3, dt, as_stream(stream)));
+}
+
+int llmhip_paged_kv_read(void *out_k, void *out_v, const void *k_pages, const void *v_pages, const int *page_table, const int *q_starts,
+                         const int *kv_lens, int tokens, int batch, int pages_per_seq, int num_pages, int page_size, int64_t page_stride,
+                         int kv_head_num, int head_dim, int cache_dt, int dt, void *stream) {
+  if (!out_k || !out_v || !k_pages || !v_pages || !all_aligned16(out_k, out_v, k_pages, v_pages)) return LLMHIP_ERR_INVALID_ARG;
+  PagedBatch b;
+  const int rc = paged_common(b, page_table, q_starts, kv_lens, tokens, batch, pages_per_seq, num_pages, page_size, page_stride, kv_head_num,
+                              head_dim, cache_dt, dt);
+  if (rc != LLMHIP_OK) return rc;
+  return from_hip(launch_paged_read(out_k, out_v, k_pages, v_pages, b, kv_head_num, cache_dt == LLMHIP_DT_FLOAT8_E4M3, dt, as_stream(stream)));
+}
+
+size_t llmhip_paged_flash_attn_workspace_bytes(int tokens, int batch, int max_q_len, int max_kv_len, int window, int sinks, int group_size,
+                                               int kv_head_num, int head_dim) {
+  if (tokens < 1 || batch < 1 || max_q_len < 1 || max_kv_len < 0 || sinks < 0 || group_size < 1 || kv_head_num < 1 || head_dim != 128) return 0;
+  if ((long long)group_size * kv_head_num > 65535) return 0;
+  return paged_attn_workspace_bytes(tokens, batch, max_q_len, max_kv_len, window > 0 ? window : 0, sinks, group_size, kv_head_num);
+}
+
+int llmhip_paged_flash_attn_gqa(void *out, const void *q, const void *k_pages, const void *v_pages, const int *page_table, const int *q_starts,
+                                const int *kv_lens, void *workspace, size_t workspace_bytes, int tokens, int batch, int max_q_len,
+                                int max_kv_len, int pages_per_seq, int num_pages, int page_size, int64_t page_stride, int window,
+                                int sinks, int group_size, int kv_head_num, int head_dim, int cache_dt, int dt, void *stream) {
+  if (!out || !q || !k_pages || !v_pages || !all_aligned16(out, q, k_pages, v_pages, workspace)) return LLMHIP_ERR_INVALID_ARG;
+  if (max_q_len < 1 || max_kv_len < 0 || sinks < 0 || group_size < 1) return LLMHIP_ERR_INVALID_ARG;
+  PagedBatch b;
+  const int rc = paged_common(b, page_table, q_starts, kv_lens, tokens, batch, pages_per_seq, num_pages, page_size, page_stride, kv_head_num,
+                              head_dim, cache_dt, dt);
+  if (rc != LLMHIP_OK) return rc;
+  // 32-bit rows of a sequence
+  if ((long long)group_size * kv_head_num > 65535 || (long long)tokens * group_size > kMaxPagedKeys) return LLMHIP_ERR_UNSUPPORTED;
+  window = window <= 0 ? 0 : window < kMaxPagedKeys ? window : kMaxPagedKeys;  // (no sequence has more keys)
+  if (sinks > kMaxPagedKeys) sinks = kMaxPagedKeys;
+  const size_t need = llmhip_paged_flash_attn_workspace_bytes(tokens, batch, max_q_len, max_kv_len, window, sinks, group_size, kv_head_num, head_dim);
+  if (need && (!workspace || workspace_bytes < need)) return LLMHIP_ERR_WORKSPACE;
+  return from_hip(launch_paged_attn(out, q, k_pages, v_pages, b, workspace, max_q_len, max_kv_len, window, sinks, group_size, kv_head_num,
+                                    cache_dt == LLMHIP_DT_FLOAT8_E4M3, dt, as_stream(stream)));
 }
 
 /* ---------------- runtime surface ---------------- */

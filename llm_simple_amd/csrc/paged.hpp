@@ -1,0 +1,89 @@
+// A KV cache in pages: where a sequence's rows are, and the 8-bit form of a row.
+//
+// K and V each have a pool of pages, page_stride bytes apart.  A page holds [kv head][page_size] rows of 128, so that the 16 keys of
+// a matrix instruction are one piece of 4 KiB (2 KiB in 8 bits), and in 8 bits behind them [kv head][page_size] exponent bytes.
+// page_size is a multiple of 16: 16 keys that begin at a multiple of 16 are in one page.
+//
+// 8 bits: x = e4m3 * 2^(byte - 127), the byte of each row the least one with max|x| <= 448 * 2^(byte - 127), at least 64.  A power of two,
+// because then nothing but the rounding to e4m3 is lost: division by the scale, and the product on the way back, are exact, and a
+// conversion instruction takes the scale along.  (Below 2^-63 a row is as good as zero: the floor keeps all of it away from subnormals.)
+//
+// Lengths, starts and the page table are device memory that a captured graph may see change: the kernels trust none of it.  A page
+// number outside of the pool, or beyond the table, is a page that is not there: its keys are not seen, rows for it are not written.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "common.hpp"
+
+namespace LLMHIP_NS {
+
+constexpr int kPageGroup = 16;  // keys that are in one page whatever its size
+
+// [rows of the dense tensors] q_starts[b] .. q_starts[b + 1] are the last rows of the kv_lens[b] cached ones of sequence b.
+struct PagedBatch {
+  const int *page_table, *q_starts, *kv_lens;
+  int batch, tokens, pages_per_seq, num_pages;
+  int keys_max;  // pages_per_seq * page_size, at most 2^31 - 2^16
+  FastDiv page_size;
+  int64_t page_stride;
+};
+
+__host__ __device__ constexpr int cached_row_bytes(bool eight) { return eight ? kHeadDim : kRowBytes; }
+
+// Where a key's row is.  page < 0: nowhere.
+struct PagePlace {
+  int page, row;
+};
+__device__ __forceinline__ PagePlace page_place(const PagedBatch &p, int b, int key) {
+  const int i = (int)fast_div(key, p.page_size);
+  PagePlace at = {-1, key - i * (int)p.page_size.d};
+  if (key >= 0 && i < p.pages_per_seq) at.page = p.page_table[(size_t)b * p.pages_per_seq + i];
+  if ((uint32_t)at.page >= (uint32_t)p.num_pages) at.page = -1;
+  return at;
+}
+
+// Whether a sequence's rows and length are such as to be worked on
+__device__ __forceinline__ bool sequence_ok(const PagedBatch &p, int first, int end, int len) {
+  return first >= 0 && first <= end && end <= p.tokens && len >= 0 && len <= p.keys_max;
+}
+
+// The sequence that a token belongs to, the same one to all lanes of the wave, or batch: how many of the sequences end before or at it.
+__device__ __forceinline__ int sequence_of(const PagedBatch &p, int token, int lane) {
+  int b = 0;
+  for (int base = 0; base < p.batch; base += 64) {
+    const int i = base + lane;
+    const bool past = i < p.batch && p.q_starts[min(i, p.batch - 1) + 1] <= token;
+    const int count = __builtin_popcountll(__builtin_amdgcn_ballot_w64(past));
+    b += count;
+    if (count < 64) break;
+  }
+  return __builtin_amdgcn_readfirstlane(b);
+}
+
+// ---- the 8-bit form ----
+
+constexpr int kLeastExponent = 64;
+// Magnitudes above the largest that has four significant bits in the storage type count as that one, so that what the 8 bits stand for is
+// in the type.  (1.875 * 2^15, 1.875 * 2^127)
+template <typename T> __device__ __forceinline__ constexpr float most_cached() { return std::is_same<T, _Float16>::value ? 61440.0f : 3.190147190316315e38f; }
+// The exponent byte of a row whose largest finite magnitude is `most`: 448 = 1.75 * 2^8, so a mantissa above 1.75 takes one more.
+__device__ __forceinline__ int exponent_byte(float most) {
+  const int e = (int)((__builtin_bit_cast(uint32_t, most) + 0x1FFFFFu) >> 23) - 8;
+  return max(e, kLeastExponent);
+}
+__device__ __forceinline__ float power_of_two(int byte) { return __builtin_bit_cast(float, (uint32_t)byte << 23); }
+
+// Two e4m3 of the low or high half of a word, times a power of two, as two values of the storage type
+template <typename T, bool HIGH> __device__ __forceinline__ uint32_t widen_pair(uint32_t word, float scale) {
+  if constexpr (std::is_same<T, _Float16>::value)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, scale, HIGH));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, scale, HIGH));
+}
+// 8 e4m3 -> 8 values of the storage type
+template <typename T> __device__ __forceinline__ u32x4_t widen8(uint32_t lo, uint32_t hi, float scale) {
+  return u32x4_t{widen_pair<T, false>(lo, scale), widen_pair<T, true>(lo, scale), widen_pair<T, false>(hi, scale), widen_pair<T, true>(hi, scale)};
+}
+
+}  // namespace LLMHIP_NS

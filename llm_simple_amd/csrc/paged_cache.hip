@@ -1,0 +1,165 @@
+// Rows into a cache of pages, rotated and in 8 bits if the cache is, and back out of it.  gfx950.
+//
+//   append:  out_q[t] = rope(in_q[t], position p of token t);  K[p] = store(rope(in_k[t], p));  V[p] = store(in_v[t])
+//   read:    out_k[t] = widen(K[p]), out_v[t] = widen(V[p]);  zeros where there is no such row
+//
+// with p = kv_lens[b] - q_starts[b + 1] + t for the tokens t of sequence b, store() and widen() the identity in a 16-bit cache and the
+// 8-bit form of paged.hpp otherwise.  The rotation is that of rope_kv_append.hip (every product and sum rounded on its own, this file is
+// compiled with -ffp-contract=off; then once to the storage type), and 8 bits are taken of its result: what the cache holds does
+// not depend on whether a row went in at once or by way of a 16-bit cache.
+#include <type_traits>
+
+#include "common.hpp"
+#include "kernels.hpp"
+#include "lanes.hpp"
+#include "paged.hpp"
+#include "rotate.hpp"
+
+namespace llmhip {
+
+struct PagedAppend {
+  PagedBatch batch;
+  char *out_q, *k_pages, *v_pages;
+  const char *in_q, *in_k, *in_v;
+  const float *freq_cis;
+  int table_rows, q_heads, kv_heads;
+};
+
+// e4m3 of 8 values of the storage type, scaled; not finite: NaN.
+template <typename T> __device__ __forceinline__ u32x2_t narrow8(const float (&x)[8], float scale) {
+  u32x2_t out;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int w = 0;
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i] * scale, x[4 * i + 1] * scale, w, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2] * scale, x[4 * i + 3] * scale, w, true);
+    out[i] = (uint32_t)w;
+  }
+  return out;
+}
+// 8 values as floats, limited; the largest finite magnitude goes into `most`
+template <typename T> __device__ __forceinline__ void limited8(u32x4_t v, float (&x)[8], float &most) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float f = Elem<T>::widen((uint16_t)(v[i >> 1] >> ((i & 1) * 16)));
+    const bool finite = __builtin_fabsf(f) < INFINITY;
+    x[i] = finite ? __builtin_amdgcn_fmed3f(f, -most_cached<T>(), most_cached<T>()) : __builtin_nanf("");
+    most = fmaxf(most, finite ? __builtin_fabsf(x[i]) : 0.0f);
+  }
+}
+
+template <typename T, bool NEOX, bool EIGHT> __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend p) {
+  const int token = blockIdx.x, tid = threadIdx.x, lane = tid & 63, j = tid & 7;
+  const int b = sequence_of(p.batch, token, lane);
+  if (b >= p.batch.batch) return;
+  const int first = p.batch.q_starts[b], end = p.batch.q_starts[b + 1], len = p.batch.kv_lens[b];
+  const int pos = len - end + token;
+  if (token < first || !sequence_ok(p.batch, first, end, len) || pos < 0 || pos >= p.table_rows) return;
+  const PagePlace at = page_place(p.batch, b, pos);
+  const int rows = p.q_heads + 2 * p.kv_heads, page_rows = (int)p.batch.page_size.d;
+  const float *tab = p.freq_cis + (size_t)pos * kHeadDim + (NEOX ? 16 : 8) * j;
+  f32x4_t cs[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) cs[i] = *reinterpret_cast<const f32x4_t *>(tab + (NEOX ? 4 * i : 64 * (i >> 1) + 4 * (i & 1)));
+  for (int r = blockIdx.y * 32 + (tid >> 3); r < rows; r += 32 * gridDim.y) {
+    const bool is_q = r < p.q_heads, is_v = r >= p.q_heads + p.kv_heads;
+    const int h = is_q ? r : r - p.q_heads - (is_v ? p.kv_heads : 0);
+    const char *in = (is_q ? p.in_q + ((size_t)token * p.q_heads + h) * kRowBytes : (is_v ? p.in_v : p.in_k) + ((size_t)token * p.kv_heads + h) * kRowBytes) + j * 16;
+    u32x4_t va = global_load_b128(in), vb = global_load_b128(in + 128);
+    if (!is_v) rotate8<T, NEOX>(va, vb, cs);
+    if (is_q) {
+      char *out = p.out_q + ((size_t)token * p.q_heads + h) * kRowBytes + j * 16;
+      store_device_b128(out, va);
+      store_device_b128(out + 128, vb);
+      continue;
+    }
+    if (at.page < 0) continue;
+    char *page = (is_v ? p.v_pages : p.k_pages) + (int64_t)at.page * p.batch.page_stride;
+    const int row = h * page_rows + at.row;
+    if constexpr (!EIGHT) {
+      char *out = page + (size_t)row * kRowBytes + j * 16;
+      store_device_b128(out, va);
+      store_device_b128(out + 128, vb);
+    } else {
+      float x[8], y[8], most = 0.0f;
+      limited8<T>(va, x, most);
+      limited8<T>(vb, y, most);
+      most = max_of_lanes<8>(most);
+      const int byte = exponent_byte(most);
+      const float scale = power_of_two(254 - byte);
+      char *out = page + (size_t)row * kHeadDim + j * 8;
+      *reinterpret_cast<u32x2_t *>(out) = narrow8<T>(x, scale);
+      *reinterpret_cast<u32x2_t *>(out + 64) = narrow8<T>(y, scale);
+      if (j == 0) page[(size_t)p.kv_heads * page_rows * kHeadDim + row] = (char)byte;
+    }
+  }
+}
+
+hipError_t launch_paged_append(void *out_q, void *k_pages, void *v_pages, const PagedBatch &batch, const void *freq_cis, const void *in_q,
+                               const void *in_k, const void *in_v, int table_rows, int q_heads, int kv_heads, int is_neox, bool eight,
+                               int dt, hipStream_t stream) {
+  const PagedAppend p = {batch,
+                         static_cast<char *>(out_q),
+                         static_cast<char *>(k_pages),
+                         static_cast<char *>(v_pages),
+                         static_cast<const char *>(in_q),
+                         static_cast<const char *>(in_k),
+                         static_cast<const char *>(in_v),
+                         static_cast<const float *>(freq_cis),
+                         table_rows,
+                         q_heads,
+                         kv_heads};
+  auto kernel_of = [&](auto t) {
+    using T = decltype(t);
+    if (eight) return is_neox ? paged_append_kernel<T, true, true> : paged_append_kernel<T, false, true>;
+    return is_neox ? paged_append_kernel<T, true, false> : paged_append_kernel<T, false, false>;
+  };
+  return launch(dt == kDtFloat16 ? kernel_of(_Float16()) : kernel_of(__bf16()), dim3(batch.tokens), 256, 0, stream, p);
+}
+
+struct PagedRead {
+  PagedBatch batch;
+  char *out_k, *out_v;
+  const char *k_pages, *v_pages;
+  int kv_heads;
+};
+
+template <typename T, bool EIGHT> __global__ __launch_bounds__(256) void paged_read_kernel(PagedRead p) {
+  const int token = blockIdx.x, tid = threadIdx.x, lane = tid & 63, j = tid & 15;
+  const int b = sequence_of(p.batch, token, lane);
+  if (b >= p.batch.batch) return;
+  const int first = p.batch.q_starts[b], end = p.batch.q_starts[b + 1], len = p.batch.kv_lens[b];
+  if (token < first || !sequence_ok(p.batch, first, end, len)) return;
+  const PagePlace at = page_place(p.batch, b, len - end + token);
+  const int page_rows = (int)p.batch.page_size.d;
+  for (int r = tid >> 4; r < 2 * p.kv_heads; r += 16) {
+    const bool is_v = r >= p.kv_heads;
+    const int h = r - (is_v ? p.kv_heads : 0);
+    u32x4_t v = {0u, 0u, 0u, 0u};
+    if (at.page >= 0) {
+      const char *page = (is_v ? p.v_pages : p.k_pages) + (int64_t)at.page * p.batch.page_stride;
+      const int row = h * page_rows + at.row;
+      if constexpr (EIGHT) {
+        const u32x2_t w = *reinterpret_cast<const u32x2_t *>(page + (size_t)row * kHeadDim + j * 8);
+        v = widen8<T>(w[0], w[1], power_of_two((uint8_t)page[(size_t)p.kv_heads * page_rows * kHeadDim + row]));
+      } else {
+        v = global_load_b128(page + (size_t)row * kRowBytes + j * 16);
+      }
+    }
+    *reinterpret_cast<u32x4_t *>((is_v ? p.out_v : p.out_k) + ((size_t)token * p.kv_heads + h) * kRowBytes + j * 16) = v;
+  }
+}
+
+hipError_t launch_paged_read(void *out_k, void *out_v, const void *k_pages, const void *v_pages, const PagedBatch &batch, int kv_heads, bool eight,
+                             int dt, hipStream_t stream) {
+  const PagedRead p = {batch,
+                       static_cast<char *>(out_k),
+                       static_cast<char *>(out_v),
+                       static_cast<const char *>(k_pages),
+                       static_cast<const char *>(v_pages),
+                       kv_heads};
+  auto kernel_of = [&](auto t) { return eight ? paged_read_kernel<decltype(t), true> : paged_read_kernel<decltype(t), false>; };
+  return launch(dt == kDtFloat16 ? kernel_of(_Float16()) : kernel_of(__bf16()), dim3(batch.tokens), 256, 0, stream, p);
+}
+
+}  // namespace llmhip

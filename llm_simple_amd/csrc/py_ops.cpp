@@ -29,7 +29,7 @@ union Value {
   void *p;
   long long i;
 };
-constexpr int kMaxArgs = 16;
+constexpr int kMaxArgs = 31;  // (one bit each in parse)
 
 bool to_value(PyObject *o, Kind kind, Value *out) {
   if (kind == B) {
@@ -193,6 +193,34 @@ OPERATOR(hip_rope_kv_append_layer,
          {"input_k_dev", P}, {"input_v_dev", P}, {"start_pos", I}, {"cur_size", I}, {"n_heads", I}, {"n_kv_heads", I},
          {"head_dim", I}, {"is_neox_style", B}, {"dt", I}, {"stream", S})
 
+OPERATOR(hip_paged_rope_kv_append_layer,
+         llmhip_paged_rope_kv_append(v[0].p, v[1].p, v[2].p, (const int *)v[3].p, (const int *)v[4].p, (const int *)v[5].p, v[6].p, v[7].p,
+                                     v[8].p, v[9].p, as_int(v[10]), as_int(v[11]), as_int(v[12]), as_int(v[13]), as_int(v[14]), v[15].i,
+                                     as_int(v[16]), as_int(v[17]), as_int(v[18]), as_int(v[19]), as_int(v[20]), as_int(v[21]),
+                                     as_int(v[22]), v[23].p),
+         {"output_q_dev", P}, {"k_pages_dev", P}, {"v_pages_dev", P}, {"page_table_dev", P}, {"q_starts_dev", P}, {"kv_lens_dev", P},
+         {"freqs_cis_dev", P}, {"input_q_dev", P}, {"input_k_dev", P}, {"input_v_dev", P}, {"tokens", I}, {"batch", I},
+         {"pages_per_seq", I}, {"num_pages", I}, {"page_size", I}, {"page_stride", L}, {"table_rows", I}, {"n_heads", I},
+         {"n_kv_heads", I}, {"head_dim", I}, {"is_neox_style", B}, {"cache_dt", I}, {"dt", I}, {"stream", S})
+
+OPERATOR(hip_paged_flash_attn_gqa_layer,
+         llmhip_paged_flash_attn_gqa(v[0].p, v[1].p, v[2].p, v[3].p, (const int *)v[4].p, (const int *)v[5].p, (const int *)v[6].p, v[7].p,
+                                     (size_t)v[8].i, as_int(v[9]), as_int(v[10]), as_int(v[11]), as_int(v[12]), as_int(v[13]),
+                                     as_int(v[14]), as_int(v[15]), v[16].i, as_int(v[17]), as_int(v[18]), as_int(v[19]), as_int(v[20]),
+                                     as_int(v[21]), as_int(v[22]), as_int(v[23]), v[24].p),
+         {"output_dev", P}, {"q_dev", P}, {"k_pages_dev", P}, {"v_pages_dev", P}, {"page_table_dev", P}, {"q_starts_dev", P},
+         {"kv_lens_dev", P}, {"workspace_dev", P}, {"workspace_bytes", L}, {"tokens", I}, {"batch", I}, {"max_q_len", I},
+         {"max_kv_len", I}, {"pages_per_seq", I}, {"num_pages", I}, {"page_size", I}, {"page_stride", L}, {"window", I}, {"sinks", I},
+         {"group_size", I}, {"kv_head_num", I}, {"head_dim", I}, {"cache_dt", I}, {"dt", I}, {"stream", S})
+
+OPERATOR(hip_paged_kv_read_layer,
+         llmhip_paged_kv_read(v[0].p, v[1].p, v[2].p, v[3].p, (const int *)v[4].p, (const int *)v[5].p, (const int *)v[6].p, as_int(v[7]),
+                              as_int(v[8]), as_int(v[9]), as_int(v[10]), as_int(v[11]), v[12].i, as_int(v[13]), as_int(v[14]),
+                              as_int(v[15]), as_int(v[16]), v[17].p),
+         {"output_k_dev", P}, {"output_v_dev", P}, {"k_pages_dev", P}, {"v_pages_dev", P}, {"page_table_dev", P}, {"q_starts_dev", P},
+         {"kv_lens_dev", P}, {"tokens", I}, {"batch", I}, {"pages_per_seq", I}, {"num_pages", I}, {"page_size", I}, {"page_stride", L},
+         {"kv_head_num", I}, {"head_dim", I}, {"cache_dt", I}, {"dt", I}, {"stream", S})
+
 PyObject *set_error(PyObject *, PyObject *cls) {
   Py_INCREF(cls);
   Py_XDECREF(g_error);
@@ -249,6 +277,22 @@ PyMethodDef methods[] = {
            "cur_size, n_heads, n_kv_heads, head_dim, is_neox_style, dt, stream=0)",
            "rope(Q), rope(K) -> k_cache[start_pos:], V -> v_cache[start_pos:] in one launch\n"
            "(src/llama2_layer_npu.cpp:790-798 + :830-844)."),
+    METHOD(hip_paged_rope_kv_append_layer,
+           "(output_q_dev, k_pages_dev, v_pages_dev, page_table_dev, q_starts_dev, kv_lens_dev, freqs_cis_dev, input_q_dev, input_k_dev, "
+           "input_v_dev, tokens, batch, pages_per_seq, num_pages, page_size, page_stride, table_rows, n_heads, n_kv_heads, head_dim, "
+           "is_neox_style, cache_dt, dt, stream=0)",
+           "rope(Q), rope(K) and V of a batch's new tokens -> their places in the pages, in 8 bits if the cache is\n"
+           "(no counterpart in the reference header)."),
+    METHOD(hip_paged_flash_attn_gqa_layer,
+           "(output_dev, q_dev, k_pages_dev, v_pages_dev, page_table_dev, q_starts_dev, kv_lens_dev, workspace_dev, workspace_bytes, "
+           "tokens, batch, max_q_len, max_kv_len, pages_per_seq, num_pages, page_size, page_stride, window, sinks, group_size, "
+           "kv_head_num, head_dim, cache_dt, dt, stream=0)",
+           "Attention of a batch's new tokens over the pages: all keys up to a token, or a window of them and the\n"
+           "first `sinks` (no counterpart in the reference header)."),
+    METHOD(hip_paged_kv_read_layer,
+           "(output_k_dev, output_v_dev, k_pages_dev, v_pages_dev, page_table_dev, q_starts_dev, kv_lens_dev, tokens, batch, "
+           "pages_per_seq, num_pages, page_size, page_stride, kv_head_num, head_dim, cache_dt, dt, stream=0)",
+           "Rows of the pages -> dense tensors (no counterpart in the reference header)."),
     {"set_error", set_error, METH_O, "The exception class of a failed call."},
     {nullptr, nullptr, 0, nullptr}};
 

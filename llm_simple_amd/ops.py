@@ -15,6 +15,7 @@ import numpy as np
 
 DT_FLOAT16 = 4   # prebuild/defs.hpp:13
 DT_BFLOAT16 = 5  # prebuild/defs.hpp:14
+DT_FLOAT8_E4M3 = 16  # of a cache in pages only; not one of the reference's types
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libllmhip.so")
@@ -35,6 +36,11 @@ SYMBOLS = {
     "llmhip_rope": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "llmhip_rope_single": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "llmhip_rope_kv_append": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "llmhip_paged_page_bytes": (_sz, [_i] * 4),
+    "llmhip_paged_rope_kv_append": (_i, [_vp] * 10 + [_i] * 5 + [_i64] + [_i] * 7 + [_vp]),
+    "llmhip_paged_flash_attn_gqa": (_i, [_vp] * 8 + [_sz] + [_i] * 7 + [_i64] + [_i] * 7 + [_vp]),
+    "llmhip_paged_flash_attn_workspace_bytes": (_sz, [_i] * 9),
+    "llmhip_paged_kv_read": (_i, [_vp] * 7 + [_i] * 5 + [_i64] + [_i] * 4 + [_vp]),
     "llmhip_matmul": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "llmhip_matmul_bias": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "llmhip_add": (_i, [_vp, _vp, _vp, ctypes.c_longlong, _i, _vp]),
@@ -115,6 +121,9 @@ from ._operators import (  # noqa: E402
     hip_flash_decode_gqa_static_layer,
     hip_matmul_bias_layer,
     hip_matmul_layer,
+    hip_paged_flash_attn_gqa_layer,
+    hip_paged_kv_read_layer,
+    hip_paged_rope_kv_append_layer,
     hip_rope_kv_append_layer,
     hip_rope_layer,
     hip_rope_single_layer,
@@ -130,6 +139,17 @@ def flash_decode_default_splits(batch, n, kv_head_num):
     """The split count of a decode call with num_splits <= 0 and up to 7 query heads per kv head (8 to 16: over a short
     cache perhaps fewer)."""
     return lib.llmhip_flash_decode_default_splits(batch, n, kv_head_num)
+
+
+def paged_page_bytes(page_size, kv_head_num, head_dim, cache_dt):
+    """Bytes of a page of K, or of V; 0 for sizes that the calls refuse."""
+    return lib.llmhip_paged_page_bytes(page_size, kv_head_num, head_dim, cache_dt)
+
+
+def paged_flash_attn_workspace_bytes(tokens, batch, max_q_len, max_kv_len, window, sinks, group_size, kv_head_num, head_dim):
+    """Workspace of hip_paged_flash_attn_gqa_layer for the same arguments."""
+    return lib.llmhip_paged_flash_attn_workspace_bytes(tokens, batch, max_q_len, max_kv_len, window, sinks, group_size, kv_head_num,
+                                                       head_dim)
 
 
 def device_props(device=0):
