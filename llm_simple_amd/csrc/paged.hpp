@@ -31,15 +31,15 @@ struct PagedBatch {
 
 __host__ __device__ constexpr int cached_row_bytes(bool eight) { return eight ? kHeadDim : kRowBytes; }
 
-// Where a key's row is.  page < 0: nowhere.
+// Where a key's row is.  page: as it stands in the table, nothing waits for the load before there() asks; -1 past the table.
 struct PagePlace {
   int page, row;
+  __device__ __forceinline__ bool there(const PagedBatch &p) const { return (uint32_t)page < (uint32_t)p.num_pages; }
 };
 __device__ __forceinline__ PagePlace page_place(const PagedBatch &p, int b, int key) {
   const int i = (int)fast_div(key, p.page_size);
   PagePlace at = {-1, key - i * (int)p.page_size.d};
   if (key >= 0 && i < p.pages_per_seq) at.page = p.page_table[(size_t)b * p.pages_per_seq + i];
-  if ((uint32_t)at.page >= (uint32_t)p.num_pages) at.page = -1;
   return at;
 }
 

@@ -15,9 +15,9 @@
 // 8-bit rows become rows of the storage type on their way into LDS: each is widened once for all rows that use it, by a conversion
 // that takes the row's power of two along, and everything after is the same code.
 //
-// Which sequence a workgroup is for is found on the device (lengths may change between replays of a graph): a wave looks at 64 sequences
-// at a time.  The keys of a sequence are dealt to as many workgroups as there are pieces of `chunk` units in what its rows see, up to the
-// launch's number of splits; then each leaves an fp32 partial, and a second launch folds them.  A unit is 128 keys (few rows) or 64.
+// What a workgroup is for is found on the device (lengths may change between replays of a graph), see find_work: a wave looks at 64 sequences
+// at a time.  Where the keys that a tile's rows see are dealt to several workgroups, each leaves an fp32 partial, and a second launch folds
+// them.  A unit of keys is 128 (few rows) or 64.
 //
 // Keys that a row must not see: their scores become -inf, so their K does not matter, but a weight of 0 times a V that is not finite
 // would be NaN.  Rows behind the last key, and pages that are not there, are zeros (the loads' descriptors end before them).  V of keys
@@ -41,69 +41,36 @@ constexpr int kUnitBytes = kTileUnit * kRowBytes;
 constexpr int kWaveStage = 32 * kRowBytes;  // staging of a few-rows wave, for K and for V
 constexpr int kPagedLds = 64 * 1024;
 
+// One kind of work of a launch
+struct PagedKind {
+  float *o, *ml;     // partials [slot][kv head][row][128], and [2]: maximum (times scale and log2 e), sum
+  int slots;         // room for so many; 0: nothing is split
+  int least;         // units that a split has at least
+  float share;       // kv heads over the workgroups that the keys are dealt to
+};
 struct PagedAttn {
   PagedBatch batch;
   char *out;
   const char *q, *k, *v;
-  float *few_o, *few_ml, *tile_o, *tile_ml;  // [tile][kv head][split][row][128], and [2]: maximum (times scale and log2 e), sum
+  PagedKind few, tiles;
   int H, Hkv, g;
-  FastDiv g_div, Hkv_div, few_splits_div, tile_splits_div;
+  FastDiv g_div, Hkv_div;
   int window, sinks;  // window 0: none
   int max_q_len;
-  int few_rows;  // sequences of up to so many rows are few-rows ones; 0: none is
+  int few_rows;    // sequences of up to so many rows are few-rows ones; 0: none is
   int few_blocks;  // workgroups of the first kind in a launch of both
-  int few_splits, few_chunk, tile_splits, tile_chunk;
 };
 
-// What a workgroup works on: `rows` rows from row `row0` of a sequence on
-struct PagedTile {
-  int b, start, m, len, row0, rows;
-};
-
-// Inclusive sum over the lanes of a wave
-__device__ __forceinline__ int wave_prefix(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15, into rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31, into rows 2 and 3
-  return x;
-}
-
-// Tile `w` of all tiles of one kind, a sequence's last (longest) one first.  False: there are not so many.
-template <bool FEW> __device__ __forceinline__ bool find_tile(const PagedAttn &p, int w, int lane, PagedTile &t) {
-  for (int base = 0; base < p.batch.batch; base += 64) {
-    const int i = min(base + lane, p.batch.batch - 1);
-    const int start = p.batch.q_starts[i], end = p.batch.q_starts[i + 1], len = p.batch.kv_lens[i];
-    const bool valid = base + lane < p.batch.batch && sequence_ok(p.batch, start, end, len) && end - start <= p.max_q_len;
-    const int m = valid ? end - start : 0, rows = m * p.g;
-    const int mine = FEW ? (m > 0 && rows <= p.few_rows ? 1 : 0) : rows <= p.few_rows ? 0 : (rows + kTileRows - 1) / kTileRows;
-    const int upto = wave_prefix(mine), all = __builtin_amdgcn_readlane(upto, 63);
-    if (w >= all) {
-      w -= all;
-      continue;
-    }
-    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > w));
-    t.b = base + l;
-    t.start = __builtin_amdgcn_readlane(start, l);
-    t.m = __builtin_amdgcn_readlane(m, l);
-    t.len = __builtin_amdgcn_readlane(len, l);
-    // 0 for the last tile (a few-rows sequence has one)
-    const int at = w - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(mine, l));
-    t.row0 = FEW ? 0 : (__builtin_amdgcn_readlane(mine, l) - 1 - at) * kTileRows;
-    t.rows = min(t.m * p.g - t.row0, FEW ? kFewCols : kTileRows);
-    return true;
-  }
-  return false;
-}
+__device__ __forceinline__ float bits_to_float(int x) { return __builtin_bit_cast(float, x); }
+__device__ __forceinline__ int float_to_bits(float x) { return __builtin_bit_cast(int, x); }
 
 // The keys that rows at positions p0 .. p1 see, in units of UNIT keys: the first `sink_units` of them are keys 0 .. sink_end, the rest
 // begin at key `first`, a multiple of 16, and end at `end`.
 struct PagedKeys {
   int sink_units, sink_end, first, end, units;
   __device__ __forceinline__ int base(int unit, int size) const { return unit < sink_units ? unit * size : first + (unit - sink_units) * size; }
-  __device__ __forceinline__ int limit(int unit) const { return unit < sink_units ? sink_end : end; }
+  // (as a sum: as a choice the compiler keeps the two in memory and loads one)
+  __device__ __forceinline__ int limit(int unit) const { return end - (int)(unit < sink_units) * (end - sink_end); }
 };
 template <int UNIT> __device__ __forceinline__ PagedKeys keys_seen(const PagedAttn &p, int p0, int p1, int len) {
   PagedKeys k;
@@ -116,56 +83,151 @@ template <int UNIT> __device__ __forceinline__ PagedKeys keys_seen(const PagedAt
   return k;
 }
 
-// Units u0 .. u1 of a split, and how many splits there are
-struct PagedSplit {
-  int count, u0, u1;
-};
-__device__ __forceinline__ PagedSplit split_of(int units, int split, int splits, int chunk) {
-  PagedSplit s = {1, 0, units};
-  if (splits > 1 && units > chunk) {
-    const int want = min(splits, (units + chunk - 1) / chunk), each = (units + want - 1) / want;
-    s.count = (units + each - 1) / each;
-    s.u0 = min(split * each, units);
-    s.u1 = min(s.u0 + each, units);
-  }
-  return s;
+// Inclusive sum over the lanes of a wave
+template <typename X> __device__ __forceinline__ X wave_prefix(X x) {
+  auto from = [&](auto control, auto rows) {
+    const int v = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(control)::value, decltype(rows)::value, 0xf, false);
+    x += __builtin_bit_cast(X, v);
+  };
+  using std::integral_constant;
+  from(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());  // row_shr:1
+  from(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
+  from(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
+  from(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
+  from(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());  // row_bcast:15, into rows 1 and 3
+  from(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());  // row_bcast:31, into rows 2 and 3
+  return x;
 }
 
-// Places of 64 groups of 16 keys, one to a lane
-struct GroupPlaces {
-  int page, row;
-  __device__ __forceinline__ void look(const PagedAttn &p, int b, int key) {
-    const PagePlace at = page_place(p.batch, b, key);
-    page = at.page;
-    row = at.row;
+// What a workgroup works on: `rows` rows from row `row0` of a sequence on, and of the keys that they see part `split` of `splits`.  slot: of
+// the first part's partial.
+struct PagedTile {
+  int b, start, m, len, row0, rows, split, splits, slot;
+};
+
+// The sequences of one kind, 64 at a time, a lane each.
+template <bool FEW> struct PagedSeqs {
+  int start, m, len, tiles, units;  // units: of the last tile, which sees most
+  __device__ __forceinline__ PagedSeqs(const PagedAttn &p, int base, int lane) {
+    const int i = min(base + lane, p.batch.batch - 1), end = p.batch.q_starts[i + 1];
+    start = p.batch.q_starts[i];
+    len = p.batch.kv_lens[i];
+    const bool valid = base + lane < p.batch.batch && sequence_ok(p.batch, start, end, len) && end - start <= p.max_q_len;
+    m = valid ? end - start : 0;
+    const int rows = m * p.g;
+    tiles = FEW ? (m > 0 && rows <= p.few_rows ? 1 : 0) : rows <= p.few_rows ? 0 : (rows + kTileRows - 1) / kTileRows;
+    const int first = FEW ? 0 : (int)fast_div(max(tiles - 1, 0) * kTileRows, p.g_div);
+    units = tiles ? keys_seen<FEW ? kFewUnit : kTileUnit>(p, len - m + first, len - 1, len).units : 0;
   }
 };
-// One group of 16 keys of a kv head
-struct Group {
-  int64_t page_at;  // bytes from the pool's base to the page
-  int row;          // row among the page's rows of all kv heads
-  int have;         // rows that are there
+
+// Dealing keys to workgroups.  The units of all tiles of a kind (each counted like its sequence's last) over the workgroups there are for
+// them make a chunk; a sequence's tiles are split into as many parts as it has chunks.  That is at most one part more to a tile than there
+// are workgroups, and a sequence in parts has at least half a chunk to a part: at most twice as many partials as workgroups.  Whoever needs
+// it works it out by itself, with the same instructions, so all agree; a sequence whose partials find no room is not split.
+//
+// FOLD: the tile of number w among those that are split.  Else: the part of number w of all; a sequence's last tiles first.
+template <bool FEW, bool FOLD> __device__ __forceinline__ bool find_work(const PagedAttn &p, int w, int lane, PagedTile &t) {
+  const PagedKind &kind = FEW ? p.few : p.tiles;
+  float chunk = 0.0f;
+  if (kind.slots) {
+    for (int base = 0; base < p.batch.batch; base += 64) {
+      const PagedSeqs<FEW> s(p, base, lane);
+      chunk += bits_to_float(__builtin_amdgcn_readlane(float_to_bits(wave_prefix((float)s.tiles * (float)s.units)), 63));
+    }
+    chunk = fmaxf(chunk * kind.share, (float)kind.least);
+  }
+  int slot = 0;
+  for (int base = 0; base < p.batch.batch; base += 64) {
+    const PagedSeqs<FEW> s(p, base, lane);
+    int splits = 1;
+    if (kind.slots) splits = max((int)__builtin_ceilf((float)s.units * __builtin_amdgcn_rcpf(chunk) * (1.0f - 0x1p-20f)), 1);  // (a whole number stays one)
+    int partials = splits > 1 ? s.tiles * splits : 0;
+    const int slots_upto = slot + wave_prefix(partials);
+    if (slots_upto > kind.slots) splits = 1;
+    const int mine = FOLD ? (splits > 1 ? s.tiles : 0) : s.tiles * splits;
+    const int upto = wave_prefix(mine), all = __builtin_amdgcn_readlane(upto, 63);
+    if (w >= all) {
+      w -= all;
+      slot = __builtin_amdgcn_readlane(slots_upto, 63);
+      continue;
+    }
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > w));
+    auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+    const int at = w - (of(upto) - of(mine));
+    t.b = base + l;
+    t.start = of(s.start);
+    t.m = of(s.m);
+    t.len = of(s.len);
+    t.splits = of(splits);
+    const int tile = FOLD || t.splits == 1 ? at : at / t.splits;
+    t.split = FOLD ? 0 : at - tile * t.splits;
+    t.slot = of(slots_upto) - of(partials) + tile * t.splits;
+    t.row0 = FEW ? 0 : (of(s.tiles) - 1 - tile) * kTileRows;
+    t.rows = min(t.m * p.g - t.row0, FEW ? kFewCols : kTileRows);
+    return true;
+  }
+  return false;
+}
+
+// Units u0 .. u1 of a part
+struct PagedPart {
+  int u0, u1;
 };
-__device__ __forceinline__ Group group_of(const PagedAttn &p, const GroupPlaces &places, int lane, int kvh, int key, int limit) {
-  Group g;
-  const int page = __builtin_amdgcn_readlane(places.page, lane);
-  g.page_at = (int64_t)page * p.batch.page_stride;
-  g.row = kvh * (int)p.batch.page_size.d + __builtin_amdgcn_readlane(places.row, lane);
-  g.have = page < 0 ? 0 : min(max(limit - key, 0), kPageGroup);
-  if (g.have == 0) g.page_at = g.row = 0;
-  return g;
+__device__ __forceinline__ PagedPart part_of(const PagedTile &t, int units) {
+  if (t.splits == 1) return PagedPart{0, units};
+  const int each = (units + t.splits - 1) / t.splits, u0 = min(t.split * each, units);
+  return PagedPart{u0, min(u0 + each, units)};
+}
+
+// 64 groups of 16 keys of a kv head, one to a lane: as the table has them, nothing waits for that load before places() ...
+constexpr int kHaveShift = 27;  // rest: row among the page's rows of all kv heads (at most 65535 * 1024), and behind it how many of the 16 are there
+struct GroupLook {
+  int page;
+  uint32_t rest;
+};
+__device__ __forceinline__ GroupLook group_look(const PagedAttn &p, int b, int kvh, int key, int limit) {
+  GroupLook l = {-1, 0};
+  const int have = min(max(limit - key, 0), kPageGroup);
+  if (have > 0) {
+    const PagePlace at = page_place(p.batch, b, key);
+    l.page = at.page;
+    l.rest = (uint32_t)(kvh * (int)p.batch.page_size.d + at.row) | (uint32_t)have << kHaveShift;
+  }
+  return l;
+}
+// ... and as bytes from the pool's base on
+struct GroupPlaces {
+  uint32_t lo, hi, rest;
+};
+struct Group {  // one of them
+  uint64_t at;
+  uint32_t rest;
+  __device__ __forceinline__ int have() const { return rest >> kHaveShift; }
+  __device__ __forceinline__ uint32_t row() const { return rest & ((1u << kHaveShift) - 1); }
+};
+template <bool EIGHT> __device__ __forceinline__ GroupPlaces group_places(const PagedAttn &p, const GroupLook &l) {
+  const bool there = (uint32_t)l.page < (uint32_t)p.batch.num_pages;
+  const uint32_t row = l.rest & ((1u << kHaveShift) - 1);
+  const uint64_t at = there ? (uint64_t)((int64_t)l.page * p.batch.page_stride) + (uint64_t)row * cached_row_bytes(EIGHT) : 0;
+  return GroupPlaces{(uint32_t)at, (uint32_t)(at >> 32), there ? l.rest : 0u};
+}
+__device__ __forceinline__ Group group_at(const GroupPlaces &places, int lane) {
+  return Group{(uint64_t)(uint32_t)__builtin_amdgcn_readlane(places.hi, lane) << 32 | (uint32_t)__builtin_amdgcn_readlane(places.lo, lane),
+               (uint32_t)__builtin_amdgcn_readlane(places.rest, lane)};
 }
 template <bool EIGHT> __device__ __forceinline__ __amdgpu_buffer_rsrc_t group_buffer(const char *pool, const Group &g) {
-  return byte_buffer(pool + g.page_at + (size_t)g.row * cached_row_bytes(EIGHT), g.have * cached_row_bytes(EIGHT));
+  return byte_buffer(pool + g.at, g.have() * cached_row_bytes(EIGHT));
 }
-// The same descriptor of a 16-bit group as words, for assembly
+// The same descriptor of a 16-bit group as words, for assembly (in scalar registers, whatever the compiler makes of it)
 __device__ __forceinline__ u32x4_t group_words(const char *pool, const Group &g) {
-  const uint64_t at = reinterpret_cast<uintptr_t>(pool + g.page_at + (size_t)g.row * kRowBytes);
-  return u32x4_t{(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, (uint32_t)(g.have * kRowBytes), 0x00020000u};
+  const uint64_t at = reinterpret_cast<uintptr_t>(pool) + g.at;
+  auto scalar = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane(x); };
+  return u32x4_t{scalar((uint32_t)at), scalar((uint32_t)(at >> 32) & 0xffffu), scalar(g.have() * kRowBytes), 0x00020000u};
 }
-// Address of the exponent byte of a group's first row
+// Address of the exponent byte of a group's first row: behind the page's values, of which 128 bytes are before it for each byte of these
 __device__ __forceinline__ const uint8_t *group_exponents(const PagedAttn &p, const char *pool, const Group &g) {
-  return reinterpret_cast<const uint8_t *>(pool + g.page_at + (size_t)p.Hkv * p.batch.page_size.d * kHeadDim + g.row);
+  return reinterpret_cast<const uint8_t *>(pool + g.at - (uint64_t)g.row() * (kHeadDim - 1) + (uint64_t)((uint32_t)p.Hkv * p.batch.page_size.d) * kHeadDim);
 }
 
 __device__ __forceinline__ bool sees(const PagedAttn &p, int pos, int key) {
@@ -189,7 +251,7 @@ __device__ __forceinline__ void exact_row(const PagedAttn &p, int b, int kvh, co
       const int key = keys.base(u, UNIT) + k0 + lane;
       PagePlace at = {-1, 0};
       if (key < keys.limit(u) && sees(p, pos, key)) at = page_place(p.batch, b, key);
-      const bool visible = at.page >= 0;
+      const bool visible = at.there(p.batch);
       const int64_t page_at = visible ? (int64_t)at.page * p.batch.page_stride : 0;
       const int row = visible ? kvh * (int)p.batch.page_size.d + at.row : 0;
       float s = -INFINITY;
@@ -222,7 +284,7 @@ __device__ __forceinline__ void exact_row(const PagedAttn &p, int b, int kvh, co
       for (int d = 0; d < D; ++d) o[d] *= alpha;
       for (int i = 0; i < G; ++i) {
         const float w = __shfl(weight, i, G);
-        const int at_page = __shfl(at.page, i, G), at_row = __shfl(row, i, G);
+        const int at_page = __shfl(visible ? at.page : -1, i, G), at_row = __shfl(row, i, G);
         if (at_page < 0) continue;
         const char *v_row = p.v + (int64_t)at_page * p.batch.page_stride + (size_t)at_row * W;
         const float scale = EIGHT ? power_of_two((uint8_t)p.v[(int64_t)at_page * p.batch.page_stride + exponents + at_row]) : 1.0f;
@@ -247,14 +309,12 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const
   using E = Elem<T>;
   constexpr int kLoads = EIGHT ? 4 : 8;  // of 1 KiB, for 32 rows
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, cg = lane >> 4;
-  const int rest = (int)fast_div(unit, p.Hkv_div), kvh = unit - rest * p.Hkv;
-  const int tile = (int)fast_div(rest, p.few_splits_div), split = rest - tile * p.few_splits;
+  const int item = (int)fast_div(unit, p.Hkv_div), kvh = unit - item * p.Hkv;
   PagedTile t;
-  if (!find_tile<true>(p, tile, lane, t)) return;
+  if (!find_work<true, false>(p, item, lane, t)) return;
   const int p0 = t.len - t.m, p1 = t.len - 1;
   const PagedKeys keys = keys_seen<kFewUnit>(p, p0, p1, t.len);
-  const PagedSplit part = split_of(keys.units, split, p.few_splits, p.few_chunk);
-  if (split >= part.count) return;
+  const PagedPart part = part_of(t, keys.units);
 
   const bool col_valid = col < t.rows;
   const int c_tok = col_valid ? (int)fast_div(col, p.g_div) : 0, c_head = kvh * p.g + (col_valid ? col - c_tok * p.g : 0);
@@ -271,17 +331,15 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const
   char *vl = lds + wave * kWaveStage, *kl = lds + (4 + wave) * kWaveStage;
   u32x4_t kn[kLoads], vn[kLoads];
   int exps = 0;  // 8 bits: of K's 32 rows in the lower lanes, of V's in the upper ones
-  GroupPlaces places = {-1, 0};
   const int iters = part.u1 - part.u0;
   auto piece = [&](int it) { return keys.base(part.u0 + it, kFewUnit) + 32 * wave; };
   auto look = [&](int it) {  // 32 steps, two groups each
-    const int i = it + (lane >> 1), u = part.u0 + i, key = keys.base(u, kFewUnit) + 32 * wave + 16 * (lane & 1);
-    places.page = -1;
-    if (i < iters && key < keys.limit(u)) places.look(p, t.b, key);
+    const int i = it + (lane >> 1), u = part.u0 + i;
+    return group_look(p, t.b, kvh, keys.base(u, kFewUnit) + 32 * wave + 16 * (lane & 1), i < iters ? keys.limit(u) : 0);
   };
-  auto group = [&](int it, int half) {
-    return group_of(p, places, (it & 31) * 2 + half, kvh, piece(it) + 16 * half, keys.limit(part.u0 + it));
-  };
+  GroupLook later = {-1, 0};
+  GroupPlaces places = {0, 0, 0};
+  auto group = [&](int it, int half) { return group_at(places, (it & 31) * 2 + half); };
   auto issue = [&](const char *pool, u32x4_t (&to)[kLoads], const Group (&g)[2]) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -295,7 +353,7 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const
       const char *pool = lane < 32 ? p.k : p.v;
       const bool second = lane & 16;
       exps = 127;
-      if ((lane & 15) < (second ? g[1].have : g[0].have))
+      if ((lane & 15) < (second ? g[1].have() : g[0].have()))
         exps = *((second ? group_exponents(p, pool, g[1]) : group_exponents(p, pool, g[0])) + (lane & 15));
     }
   };
@@ -321,7 +379,9 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const
   float m_run = -INFINITY, l_run = 0.0f;
   Group now[2];
   if (iters > 0) {
-    look(0);
+    later = look(0);
+    places = group_places<EIGHT>(p, later);
+    later = look(32);
     now[0] = group(0, 0);
     now[1] = group(0, 1);
     issue(p.k, kn, now);
@@ -330,17 +390,20 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const
   }
   for (int it = 0; it < iters; ++it) {
     const int base = piece(it), limit = keys.limit(part.u0 + it);
-    const bool whole = now[0].have == kPageGroup && now[1].have == kPageGroup;
-    const bool any = now[0].have + now[1].have > 0;
+    const bool whole = now[0].have() == kPageGroup && now[1].have() == kPageGroup;
+    const bool any = now[0].have() + now[1].have() > 0;
     if (any) {
       __builtin_amdgcn_wave_barrier();
       stage(kl, kn, 0, [](int row, int granule) { return k_swizzle_off(row, granule); });
       stage(vl, vn, 1, [](int row, int granule) { return v_swizzle32_off(row, granule); });
       __builtin_amdgcn_wave_barrier();
     }
-    const bool there[2] = {now[0].have > 0, now[1].have > 0};
+    const bool there[2] = {now[0].have() > 0, now[1].have() > 0};
     if (it + 1 < iters) {
-      if (((it + 1) & 31) == 0) look(it + 1);
+      if (((it + 1) & 31) == 0) {
+        places = group_places<EIGHT>(p, later);
+        later = look(it + 33);
+      }
       now[0] = group(it + 1, 0);
       now[1] = group(it + 1, 1);
       issue(p.k, kn, now);
@@ -434,7 +497,7 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const
   const bool finite = size < INFINITY;
   if (__builtin_expect(((__builtin_amdgcn_ballot_w64(!finite) >> (lane & 48)) & 0xffff) != 0, 0))
     exact_row<T, EIGHT, 16, kFewUnit>(p, t.b, kvh, p.q + row_at, p0 + tok, keys, part.u0, part.u1, M, L, acc);
-  if (part.count == 1) {
+  if (t.splits == 1) {
     const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);  // (NaN stays NaN)
     u32x4_t w;
 #pragma unroll
@@ -442,40 +505,47 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const
     *reinterpret_cast<u32x4_t *>(p.out + row_at + dch * 16) = w;
     return;
   }
-  const size_t slot = (((size_t)tile * p.Hkv + kvh) * p.few_splits + split) * kFewCols + c;
-  float *wo = p.few_o + slot * kHeadDim + 8 * dch;
+  const size_t slot = ((size_t)(t.slot + t.split) * p.Hkv + kvh) * kFewCols + c;
+  float *wo = p.few.o + slot * kHeadDim + 8 * dch;
   *reinterpret_cast<f32x4_t *>(wo) = f32x4_t{acc[0], acc[1], acc[2], acc[3]};
   *reinterpret_cast<f32x4_t *>(wo + 4) = f32x4_t{acc[4], acc[5], acc[6], acc[7]};
-  if (dch == 0) *reinterpret_cast<float2 *>(p.few_ml + slot * 2) = float2{M, L};
+  if (dch == 0) *reinterpret_cast<float2 *>(p.few.ml + slot * 2) = float2{M, L};
 }
 
 // ---- tiles ----
 
-// 1 KiB from a descriptor into LDS, lane by lane.  Inline: the compiler would order every later LDS read behind the load; what it is for
-// is waited for where the waves meet (s_waitcnt vmcnt before a barrier).
-__device__ __forceinline__ void load_to_lds(u32x4_t r, int lane_off, uint32_t lds_at) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" : : "v"(lane_off), "s"(r), "s"(lds_at) : "m0", "memory");
+// 16 rows of a group into LDS, four times 1 KiB, lane by lane: the instruction's offset moves both addresses.  Inline: the compiler would
+// order every later LDS read behind the loads; they are waited for where the waves meet (s_waitcnt vmcnt before a barrier).
+__device__ __forceinline__ void load_group(u32x4_t r, int o0, int o1, int o2, int o3, uint32_t lds_at) {
+  asm volatile(
+      "s_mov_b32 m0, %5\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %4, 0 offen lds\n\tbuffer_load_dwordx4 %1, %4, 0 offen offset:1024 lds\n\t"
+      "buffer_load_dwordx4 %2, %4, 0 offen offset:2048 lds\n\tbuffer_load_dwordx4 %3, %4, 0 offen offset:3072 lds"
+      :
+      : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(r), "s"(lds_at)
+      : "m0", "memory");
 }
 
+// The loop is that of the prefill kernels: K runs one tile ahead of V, so that the matrix instructions of S(j + 1) = K(j + 1) Q^T stand
+// beside the softmax of tile j, and those of P(j) V(j) beside the exponentials.  In a step, K(j + 2) goes where K(j) was and V(j + 1) where
+// V(j - 1) was, both read in the step before.
 template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(const PagedAttn &p, int unit, char *lds) {
   using E = Elem<T>;
+  constexpr int kVRegion = 2 * kUnitBytes;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int rest = (int)fast_div(unit, p.Hkv_div), kvh = unit - rest * p.Hkv;
-  const int tile = (int)fast_div(rest, p.tile_splits_div), split = rest - tile * p.tile_splits;
+  const int item = (int)fast_div(unit, p.Hkv_div), kvh = unit - item * p.Hkv;
   PagedTile t;
-  if (!find_tile<false>(p, tile, lane, t)) return;
+  if (!find_work<false, false>(p, item, lane, t)) return;
   const int before = t.len - t.m;  // tokens cached before the new ones
   const int p0 = before + (int)fast_div(t.row0, p.g_div), p1 = before + (int)fast_div(t.row0 + t.rows - 1, p.g_div);
   const PagedKeys keys = keys_seen<kTileUnit>(p, p0, p1, t.len);
-  const PagedSplit part = split_of(keys.units, split, p.tile_splits, p.tile_chunk);
-  if (split >= part.count) return;
+  const PagedPart part = part_of(t, keys.units);
 
   // this wave's rows, and this lane's
   const int w_rows = min(t.rows - 32 * wave, 32), w_row0 = t.row0 + 32 * wave;  // (none: w_rows <= 0)
   const int w_p0 = w_rows > 0 ? before + (int)fast_div(w_row0, p.g_div) : 0;
   const int w_p1 = w_rows > 0 ? before + (int)fast_div(w_row0 + w_rows - 1, p.g_div) : -1;
   WaveAttn<T, 2> w;
-  w.init(lds, lane, 2 * kUnitBytes);
+  w.init(lds, lane, kVRegion);
   auto place_of = [&](int r, int &tok) {  // byte offset of row r of the wave's, in q and in out
     tok = (int)fast_div(w_row0 + r, p.g_div);
     return ((size_t)(t.start + tok) * p.H + kvh * p.g + w_row0 + r - tok * p.g) * kRowBytes;
@@ -490,99 +560,154 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
   }
   const int my_pos = before + my_tok;
 
-  // Wave i fetches group i of every tile: 16 rows of K and of V.  Lane offsets of the four loads of 4 rows (16 bits), which
-  // undo the swizzle of the LDS rows.
+  // Wave i fetches group i of every tile: 16 rows of K and of V.  Lane offsets within 4 rows (16 bits), which undo the swizzle of
+  // the LDS rows.
   const int r4 = lane >> 4, c16 = lane & 15;
   int k_off[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) k_off[i] = (4 * i + r4) * kRowBytes + ((c16 ^ (4 * i + r4)) << 4);
+  for (int i = 0; i < 4; ++i) k_off[i] = r4 * kRowBytes + ((c16 ^ (4 * i + r4)) << 4);
   const int v_off = r4 * kRowBytes + (((((c16 >> 2) ^ r4) << 2) | (c16 & 3)) << 4);
-  const uint32_t lds_k = lds_address(lds) + wave * kPageGroup * kRowBytes, lds_v = lds_k + 2 * kUnitBytes;
-  u32x4_t kn[2], vn[2];
+  const uint32_t lds_k = __builtin_amdgcn_readfirstlane(lds_address(lds) + wave * kPageGroup * kRowBytes), lds_v = lds_k + kVRegion;
+  u32x4_t kn[2], vn[2];  // 8 bits: what is on its way to slots of K and V
   int exps = 0;
 
   const int iters = part.u1 - part.u0;
-  GroupPlaces places = {-1, 0}, later = {-1, 0};
-  auto look = [&](GroupPlaces &to, int it) {  // 16 tiles, four groups each
-    const int i = it + (lane >> 2), u = part.u0 + i, key = keys.base(u, kTileUnit) + 16 * (lane & 3);
-    to.page = -1;
-    if (i < iters && key < keys.limit(u)) to.look(p, t.b, key);
+  auto look = [&](int it) {  // 16 tiles, four groups each
+    const int i = it + (lane >> 2), u = part.u0 + i;
+    return group_look(p, t.b, kvh, keys.base(u, kTileUnit) + 16 * (lane & 3), i < iters ? keys.limit(u) : 0);
   };
-  auto issue = [&](int it) {
-    const int u = part.u0 + it, key = keys.base(u, kTileUnit) + 16 * wave;
-    const Group g = group_of(p, places, (it & 15) * 4 + wave, kvh, key, keys.limit(u));
+  GroupLook later = {-1, 0};
+  GroupPlaces places = {0, 0, 0};
+  // Where this wave's group of tile `it` is, and which groups of the tile are there at all
+  struct Next {
+    Group g;
+    uint32_t there;
+  };
+  auto next_of = [&](int it) {
+    if ((it & 15) == 0) {
+      places = group_places<EIGHT>(p, later);
+      later = look(it + 16);
+    }
+    Next n;
+    n.g = group_at(places, (it & 15) * 4 + wave);
+    n.there = (uint32_t)(__builtin_amdgcn_ballot_w64(places.rest != 0) >> ((it & 15) * 4)) & 15u;
+    return n;
+  };
+  auto issue_k = [&](const Group &g, int slot) {
     if constexpr (EIGHT) {
-      const __amdgpu_buffer_rsrc_t kb = group_buffer<true>(p.k, g), vb = group_buffer<true>(p.v, g);
+      const __amdgpu_buffer_rsrc_t r = group_buffer<true>(p.k, g);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        kn[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(kb, i * 1024 + lane * 16, 0, 0));
-        vn[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(vb, i * 1024 + lane * 16, 0, 0));
-      }
-      exps = 127;
-      if ((lane & 15) < g.have && !(lane & 16)) exps = *(group_exponents(p, lane < 32 ? p.k : p.v, g) + (lane & 15));
+      for (int i = 0; i < 2; ++i) kn[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, i * 1024 + lane * 16, 0, 0));
     } else {
-      const uint32_t slot = (it & 1) * kUnitBytes;
-      const u32x4_t kb = group_words(p.k, g), vb = group_words(p.v, g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) load_to_lds(kb, k_off[i], __builtin_amdgcn_readfirstlane(lds_k + slot + i * 1024));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) load_to_lds(vb, v_off + i * 1024, __builtin_amdgcn_readfirstlane(lds_v + slot + i * 1024));
+      load_group(group_words(p.k, g), k_off[0], k_off[1], k_off[2], k_off[3], lds_k + slot * kUnitBytes);
     }
   };
-  auto widen = [&](int it) {  // 8 bits: what issue() fetched goes to LDS
-    char *k_to = lds + (it & 1) * kUnitBytes, *v_to = k_to + 2 * kUnitBytes;
+  auto issue_v = [&](const Group &g, int slot) {
+    if constexpr (EIGHT) {
+      const __amdgpu_buffer_rsrc_t r = group_buffer<true>(p.v, g);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) vn[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, i * 1024 + lane * 16, 0, 0));
+    } else {
+      load_group(group_words(p.v, g), v_off, v_off, v_off, v_off, lds_v + slot * kUnitBytes);
+    }
+  };
+  auto issue_exponents = [&](const Group &gk, const Group &gv) {  // of K's rows in lanes 0 .. 15, of V's in lanes 32 .. 47
+    if constexpr (EIGHT) {
+      const bool upper = lane & 32;
+      exps = 127;
+      if ((lane & 31) < (upper ? gv.have() : gk.have())) exps = *((upper ? group_exponents(p, p.v, gv) : group_exponents(p, p.k, gk)) + (lane & 31));
+    }
+  };
+  auto widen = [&](const u32x4_t (&from)[2], int lane0, char *to, auto place) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = 8 * i + (lane >> 3), row = 16 * wave + r, granule = 2 * (lane & 7);
-      const float ks = power_of_two(__builtin_amdgcn_ds_bpermute(4 * r, exps)), vs = power_of_two(__builtin_amdgcn_ds_bpermute(4 * (r + 32), exps));
-      lds_write_b128(k_to, k_swizzle_off(row, granule), widen8<T>(kn[i][0], kn[i][1], ks));
-      lds_write_b128(k_to, k_swizzle_off(row, granule + 1), widen8<T>(kn[i][2], kn[i][3], ks));
-      lds_write_b128(v_to, v_swizzle_off(row, granule), widen8<T>(vn[i][0], vn[i][1], vs));
-      lds_write_b128(v_to, v_swizzle_off(row, granule + 1), widen8<T>(vn[i][2], vn[i][3], vs));
+      const float scale = power_of_two(__builtin_amdgcn_ds_bpermute(4 * (r + lane0), exps));
+      lds_write_b128(to, place(row, granule), widen8<T>(from[i][0], from[i][1], scale));
+      lds_write_b128(to, place(row, granule + 1), widen8<T>(from[i][2], from[i][3], scale));
     }
   };
+  auto widen_k = [&](int slot) {
+    if constexpr (EIGHT) widen(kn, 0, lds + slot * kUnitBytes, [](int row, int granule) { return k_swizzle_off(row, granule); });
+  };
+  auto widen_v = [&](int slot) {
+    if constexpr (EIGHT) widen(vn, 32, lds + kVRegion + slot * kUnitBytes, [](int row, int granule) { return v_swizzle_off(row, granule); });
+  };
+
+  // tiles in which this wave's rows see a key
+  const int w_keys = w_p1 + 1;
+  const int w_units = w_keys > keys.first ? keys.sink_units + (w_keys - keys.first + kTileUnit - 1) / kTileUnit : (max(w_keys, 0) + kTileUnit - 1) / kTileUnit;
+  const int w_iters = max(0, min(iters, w_units - part.u0));
+  f32x16_t sa[2], sb[2];
+  Next cur = {}, nxt = {}, after = {};  // of tiles j, j + 1 and j + 2
+  float scale = kScaleLog2e;
+  asm volatile("" : "+s"(scale));
   if (iters > 0) {
-    look(places, 0);
-    issue(0);
-    if (EIGHT) widen(0);
-    look(later, 16);
-  }
-  for (int it = 0; it < iters; ++it) {
-    const int u = part.u0 + it, base = keys.base(u, kTileUnit), limit = keys.limit(u);
-    const uint64_t there = __builtin_amdgcn_ballot_w64(places.page >= 0) >> ((it & 15) * 4);
-    // the tile is there, in all waves' groups, and the other slot is free
+    later = look(0);
+    cur = next_of(0);
+    nxt = next_of(1);
+    after = next_of(2);
+    issue_k(cur.g, 0);
+    issue_v(cur.g, 0);
+    issue_exponents(cur.g, cur.g);
+    widen_k(0);
+    widen_v(0);
+    issue_k(nxt.g, 1);
+    issue_exponents(nxt.g, cur.g);
+    widen_k(1);
+    // (the compiler knows nothing of the waits below, and would wait for Q, and with it for the tiles on their way, in the loop)
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) asm volatile("" : "+v"(w.qf[kk]));
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (it + 1 < iters) {
-      if (((it + 1) & 15) == 0) {
-        places = later;
-        look(later, it + 17);
-      }
-      issue(it + 1);
-    }
-    if (base <= w_p1) {
-      f32x16_t s[2];
-      const int slot = (it & 1) * kUnitBytes;
-      w.qk(lds, slot, s);
-      if (base + kTileUnit > min(w_p0 + 1, limit) || (there & 15) != 15 || (p.window > 0 && base <= w_p1 - p.window && base + kTileUnit > p.sinks)) {
-        const int from = base + 4 * w.hh, last = min(my_pos, limit - 1) - from;
-        const int first = p.window > 0 ? my_pos - p.window - from : -(1 << 30), sink = p.sinks - from;
+    if (w_iters > 0) w.qk(lds, 0, sa);
+    // K(2) goes where tile 0 was just read: no wave may issue it before all have
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+  auto step = [&](int it, auto slot_, f32x16_t (&s)[2], f32x16_t (&s_next)[2]) {
+    constexpr int slot = decltype(slot_)::value;
+    issue_k(after.g, slot);
+    issue_v(nxt.g, slot ^ 1);
+    issue_exponents(after.g, nxt.g);
+    if (it < w_iters) {
+      const int u = part.u0 + it, base = keys.base(u, kTileUnit), limit = keys.limit(u);
+      if (base + kTileUnit > min(w_p0 + 1, limit) || cur.there != 15 || (p.window > 0 && base <= w_p1 - p.window && base + kTileUnit > p.sinks)) {
+        const int from = base + 4 * w.hh;
+        // a lane's keys are 8 * (i / 4) + i % 4 of 32 from its first one on
+        auto hide = [&](auto hidden) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+          for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int c = kb * 32 + 8 * (i >> 2) + (i & 3);
-            if (c > last || (c <= first && c >= sink) || !(there >> (2 * kb + (i >> 3)) & 1)) s[kb][i] = -INFINITY;
-          }
+            for (int i = 0; i < 16; ++i) s[kb][i] = hidden(kb * 32 + 8 * (i >> 2) + (i & 3), 2 * kb + (i >> 3)) ? -INFINITY : s[kb][i];
+        };
+        const int last = min(my_pos, limit - 1) - from;
+        hide([&](int c, int) { return c > last; });
+        if (p.window > 0) {
+          const int first = my_pos - p.window - from, sink = p.sinks - from;
+          hide([&](int c, int) { return (int)(c <= first) & (int)(c >= sink); });
+        }
+        if (cur.there != 15) hide([&](int, int group) { return !(cur.there >> group & 1); });
       }
-      w.row_max(s, kScaleLog2e);
-      w.l_run += w.probabilities(s, kScaleLog2e);
-      w.pv(slot);
+      // (the last tile's S(j + 1) is not used: a branch would part these matrix instructions from what they stand beside)
+      constexpr int next = (slot ^ 1) * kUnitBytes;
+      w.template qk<0, 3>(lds, next, s_next);
+      w.row_max(s, scale);
+      w.template qk<3, 8>(lds, next, s_next);
+      w.l_run += w.probabilities(s, scale);
+      w.pv(slot * kUnitBytes);
     }
-    if (EIGHT && it + 1 < iters) widen(it + 1);
+    widen_k(slot);
+    widen_v(slot ^ 1);
+    cur = nxt;
+    nxt = after;
+    after = next_of(it + 3);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+  for (int it = 0; it < iters; it += 2) {
+    step(it, std::integral_constant<int, 0>(), sa, sb);
+    if (it + 1 < iters) step(it + 1, std::integral_constant<int, 1>(), sb, sa);
   }
 
   // ---- rows that are not finite, key by key ----
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   char *mine = lds + wave * 32 * kRowBytes;
   float size = 0.0f;
 #pragma unroll
@@ -611,16 +736,16 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
   }
 
   const float l_tot = pair_sum(w.l_run);
-  if (part.count > 1) {
+  if (t.splits > 1) {
     if (w.l32 < w_rows) {
-      const size_t slot = (((size_t)tile * p.Hkv + kvh) * p.tile_splits + split) * kTileRows + 32 * wave + w.l32;
-      float *o_row = p.tile_o + slot * kHeadDim;
+      const size_t slot = ((size_t)(t.slot + t.split) * p.Hkv + kvh) * kTileRows + 32 * wave + w.l32;
+      float *o_row = p.tiles.o + slot * kHeadDim;
 #pragma unroll
       for (int d = 0; d < 4; ++d)
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4)
           *reinterpret_cast<f32x4_t *>(o_row + 32 * d + 8 * i4 + 4 * w.hh) = f32x4_t{w.o[d][4 * i4], w.o[d][4 * i4 + 1], w.o[d][4 * i4 + 2], w.o[d][4 * i4 + 3]};
-      if (w.hh == 0) *reinterpret_cast<float2 *>(p.tile_ml + slot * 2) = float2{w.m_run * kScaleLog2e, l_tot};
+      if (w.hh == 0) *reinterpret_cast<float2 *>(p.tiles.ml + slot * 2) = float2{w.m_run * kScaleLog2e, l_tot};
     }
     return;
   }
@@ -653,82 +778,86 @@ template <typename T, bool EIGHT, PagedMode MODE> __global__ __launch_bounds__(2
     tile_rows<T, EIGHT>(p, unit - (MODE == kBoth ? p.few_blocks : 0), lds);
 }
 
-// Partials of a (tile, kv head), 16 rows to a workgroup, 16 lanes to a row.
+// Partials of a (tile, kv head), 8 rows to a workgroup, 32 lanes of 4 dims to a row; 8 partials are on their way at a time.
 template <typename T> __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttn p) {
-  const int tid = threadIdx.x, lane = tid & 63, dch = tid & 15;
+  const int tid = threadIdx.x, lane = tid & 63, d4 = (tid & 31) * 4;
   const bool few = (int)blockIdx.x < p.few_blocks;
-  int unit = few ? blockIdx.x : blockIdx.x - p.few_blocks;
-  const int rows0 = few ? 0 : (unit & 7) * 16;
-  if (!few) unit >>= 3;
-  const int tile = (int)fast_div(unit, p.Hkv_div), kvh = unit - tile * p.Hkv;
+  const int block = few ? blockIdx.x : blockIdx.x - p.few_blocks, slot_rows = few ? kFewCols : kTileRows;
+  const int unit = block / (few ? kFewCols / 8 : kTileRows / 8), c = (block % (few ? kFewCols / 8 : kTileRows / 8)) * 8 + (tid >> 5);
+  const int item = (int)fast_div(unit, p.Hkv_div), kvh = unit - item * p.Hkv;
   PagedTile t;
-  if (!(few ? find_tile<true>(p, tile, lane, t) : find_tile<false>(p, tile, lane, t))) return;
-  const int before = t.len - t.m, p0 = before + (int)fast_div(t.row0, p.g_div), p1 = before + (int)fast_div(t.row0 + t.rows - 1, p.g_div);
-  const int units = few ? keys_seen<kFewUnit>(p, p0, p1, t.len).units : keys_seen<kTileUnit>(p, p0, p1, t.len).units;
-  const int splits = few ? p.few_splits : p.tile_splits, count = split_of(units, 0, splits, few ? p.few_chunk : p.tile_chunk).count;
-  const int c = rows0 + (tid >> 4), slot_rows = few ? kFewCols : kTileRows;
-  if (count == 1 || c >= t.rows) return;
-  const size_t slot = ((size_t)tile * p.Hkv + kvh) * splits * slot_rows + c;
-  const float *po = (few ? p.few_o : p.tile_o) + slot * kHeadDim + 8 * dch, *pml = (few ? p.few_ml : p.tile_ml) + slot * 2;
-  float M = -INFINITY, L = 0.0f, acc[8];
+  if (!(few ? find_work<true, true>(p, item, lane, t) : find_work<false, true>(p, item, lane, t))) return;
+  if (c >= t.rows) return;
+  const PagedKind &kind = few ? p.few : p.tiles;
+  const size_t row = ((size_t)t.slot * p.Hkv + kvh) * slot_rows + c, step = (size_t)p.Hkv * slot_rows;
+  const float *po = kind.o + row * kHeadDim + d4, *pml = kind.ml + row * 2;
+  float M = -INFINITY, L = 0.0f;
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  constexpr int D = 8;
+  for (int s0 = 0; s0 < t.splits; s0 += D) {
+    float2 ml[D];
+    f32x4_t o[D];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
-  for (int s = 0; s < count; ++s) M = fmaxf(M, pml[(size_t)s * slot_rows * 2]);
-  const float M_use = M == -INFINITY ? 0.0f : M;
-#pragma unroll 4
-  for (int s = 0; s < count; ++s) {
-    const float2 ml = *reinterpret_cast<const float2 *>(pml + (size_t)s * slot_rows * 2);
-    const float *row = po + (size_t)s * slot_rows * kHeadDim;
-    const f32x4_t a = *reinterpret_cast<const f32x4_t *>(row), b = *reinterpret_cast<const f32x4_t *>(row + 4);
-    const float wt = fast_exp2(ml.x - M_use);
-    L += wt * ml.y;
+    for (int j = 0; j < D; ++j) {
+      const size_t at = min(s0 + j, t.splits - 1) * step;
+      ml[j] = *reinterpret_cast<const float2 *>(pml + at * 2);
+      o[j] = *reinterpret_cast<const f32x4_t *>(po + at * kHeadDim);
+    }
+    float most = M;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      acc[j] += wt * a[j];
-      acc[4 + j] += wt * b[j];
+    for (int j = 0; j < D; ++j) most = fmaxf(most, ml[j].x);
+    const float m_use = most == -INFINITY ? 0.0f : most, before = fast_exp2(M - m_use);
+    M = most;
+    L *= before;
+    acc *= before;
+#pragma unroll
+    for (int j = 0; j < D; ++j) {
+      const float wt = s0 + j < t.splits ? fast_exp2(ml[j].x - m_use) : 0.0f;
+      if (s0 + j < t.splits) {
+        L += wt * ml[j].y;
+        acc += wt * o[j];
+      }
     }
   }
-  const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);
+  const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);  // (NaN stays NaN)
   const int tok = (int)fast_div(t.row0 + c, p.g_div);
-  u32x4_t w;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = Elem<T>::pack2(acc[2 * j] * inv, acc[2 * j + 1] * inv);
-  *reinterpret_cast<u32x4_t *>(p.out + ((size_t)(t.start + tok) * p.H + kvh * p.g + t.row0 + c - tok * p.g) * kRowBytes + dch * 16) = w;
+  const u32x2_t w = {Elem<T>::pack2(acc[0] * inv, acc[1] * inv), Elem<T>::pack2(acc[2] * inv, acc[3] * inv)};
+  *reinterpret_cast<u32x2_t *>(p.out + ((size_t)(t.start + tok) * p.H + kvh * p.g + t.row0 + c - tok * p.g) * kRowBytes + d4 * 2) = w;
 }
 
-// How a launch is cut, from what the host knows: bounds, not lengths.
+// How a launch is shaped, from what the host knows: bounds, not lengths.
 struct PagedPlan {
-  bool few, tiles;
-  long long few_tiles, row_tiles;
-  int few_splits, few_chunk, tile_splits, tile_chunk;
-  size_t few_slots() const { return few && few_splits > 1 ? (size_t)few_tiles * few_splits * kFewCols : 0; }
-  size_t tile_slots() const { return tiles && tile_splits > 1 ? (size_t)row_tiles * tile_splits * kTileRows : 0; }
-  size_t bytes(int Hkv) const { return (few_slots() + tile_slots()) * Hkv * (kHeadDim + 2) * sizeof(float); }
+  struct Kind {
+    long long tiles, items, slots, rows;  // at most; rows of a partial
+    int least;
+    float share;
+    size_t bytes(int Hkv) const { return (size_t)slots * Hkv * rows * (kHeadDim + 2) * sizeof(float); }
+    long long folds() const { return slots / 2 < tiles ? slots / 2 : tiles; }  // tiles that are split, at most
+  } few, by_tiles;
+  size_t bytes(int Hkv) const { return few.bytes(Hkv) + by_tiles.bytes(Hkv); }
 };
 static PagedPlan plan_paged(int tokens, int batch, int max_q_len, int max_kv_len, int window, int sinks, int g, int Hkv) {
   PagedPlan pl = {};
-  const long long cus = device_compute_units(), most_rows = (long long)max_q_len * g;
-  const long long sequences = batch < tokens ? batch : tokens;  // that have new tokens at all
-  pl.tiles = most_rows > kFewCols;
-  // all sequences have max_q_len tokens, or the tokens do not add up
-  pl.few = !pl.tiles || (g <= kFewCols && (long long)batch * max_q_len != tokens);
-  pl.few_tiles = sequences;
-  pl.row_tiles = (long long)tokens * g / kTileRows + sequences;
-  auto cut = [&](long long wgs, int unit, long long seen, long long target, int least, int &splits, int &chunk) {
-    const long long units = (seen + unit - 1) / unit;
-    long long s = (target + wgs - 1) / wgs;
-    if (s > (units + least - 1) / least) s = (units + least - 1) / least;
-    s = s < 1 ? 1 : s > 64 ? 64 : s;
-    chunk = units > s ? (int)((units + s - 1) / s) : 1;
-    splits = (int)((units + chunk - 1) / chunk);
-    if (splits < 1) splits = 1;
+  const long long cus = device_compute_units(), sequences = batch < tokens ? batch : tokens;  // that have new tokens at all
+  const bool tiles = (long long)max_q_len * g > kFewCols;
+  // (all sequences have max_q_len tokens, or the tokens do not add up: no few-rows ones)
+  if (!tiles || (g <= kFewCols && (long long)batch * max_q_len != tokens)) pl.few.tiles = sequences;
+  if (tiles) pl.by_tiles.tiles = (long long)tokens * g / kTileRows + sequences;
+  auto deal = [&](PagedPlan::Kind &kind, int rows, int unit, long long span, long long workgroups, int least) {
+    kind.rows = rows;
+    kind.least = least;
+    kind.share = (float)Hkv / (float)workgroups;
+    const long long windowed = (long long)window + span + sinks + 2 * kPageGroup, seen = window > 0 && windowed < max_kv_len ? windowed : max_kv_len;
+    const long long each = workgroups / Hkv + 1;
+    // in parts: not if no sequence is longer than a part's least, nor if the tiles of even one that is in parts would be more than workgroups
+    const bool parts = kind.tiles > 0 && (seen + unit - 1) / unit > least;
+    kind.slots = parts ? 2 * each + 2 : 0;
+    const long long most = kind.tiles * ((seen + unit - 1) / unit / least + 1);
+    if (kind.slots > most) kind.slots = most;
+    kind.items = kind.tiles + (kind.slots ? each + each / 64 + 1 : 0);
   };
-  auto seen = [&](long long rows_span) {
-    const long long most = (long long)window + rows_span + sinks + 2 * kPageGroup;
-    return window > 0 && most < max_kv_len ? most : (long long)max_kv_len;
-  };
-  if (pl.few) cut(pl.few_tiles * Hkv, kFewUnit, seen(kFewCols), 4 * cus, 4, pl.few_splits, pl.few_chunk);
-  if (pl.tiles) cut(pl.row_tiles * Hkv, kTileUnit, seen(kTileRows / g + 1), 2 * cus, 8, pl.tile_splits, pl.tile_chunk);
+  deal(pl.few, kFewCols, kFewUnit, kFewCols, 2 * cus, 2);
+  deal(pl.by_tiles, kTileRows, kTileUnit, kTileRows / g + 1, 2 * cus, 6);
   return pl;
 }
 
@@ -750,38 +879,32 @@ hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, cons
   p.g = g;
   p.g_div = make_fast_div(g);
   p.Hkv_div = make_fast_div(Hkv);
-  p.few_splits = pl.few ? pl.few_splits : 1;
-  p.few_chunk = pl.few_chunk;
-  p.tile_splits = pl.tiles ? pl.tile_splits : 1;
-  p.tile_chunk = pl.tile_chunk;
-  p.few_splits_div = make_fast_div(p.few_splits);
-  p.tile_splits_div = make_fast_div(p.tile_splits);
   p.window = window;
   p.sinks = sinks;
   p.max_q_len = max_q_len;
-  p.few_rows = pl.few ? kFewCols : 0;
+  p.few_rows = pl.few.tiles ? kFewCols : 0;
   float *ws = static_cast<float *>(workspace);
-  const size_t few_slots = pl.few_slots() * Hkv, tile_slots = pl.tile_slots() * Hkv;
-  p.few_o = ws;
-  p.tile_o = p.few_o + few_slots * kHeadDim;
-  p.few_ml = p.tile_o + tile_slots * kHeadDim;
-  p.tile_ml = p.few_ml + few_slots * 2;
-  const long long few_blocks = pl.few ? pl.few_tiles * Hkv * p.few_splits : 0, tile_blocks = pl.tiles ? pl.row_tiles * Hkv * p.tile_splits : 0;
-  if (few_blocks + tile_blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+  auto kind_of = [&](const PagedPlan::Kind &k) {
+    const PagedKind kind = {ws, ws + (size_t)k.slots * Hkv * k.rows * kHeadDim, (int)k.slots, k.least, k.share};
+    if (k.slots) ws += k.bytes(Hkv) / sizeof(float);
+    return kind;
+  };
+  p.few = kind_of(pl.few);
+  p.tiles = kind_of(pl.by_tiles);
+  const long long few_blocks = pl.few.items * Hkv, tile_blocks = pl.by_tiles.items * Hkv;
+  const long long few_folds = pl.few.folds() * Hkv * (kFewCols / 8), tile_folds = pl.by_tiles.folds() * Hkv * (kTileRows / 8);
+  if (few_blocks + tile_blocks > 0x7fffffffLL || few_folds + tile_folds > 0x7fffffffLL) return hipErrorInvalidValue;
   p.few_blocks = (int)few_blocks;
   auto kernel_of = [&](auto mode) {
     constexpr PagedMode MODE = decltype(mode)::value;
     if (dt == kDtFloat16) return eight ? paged_attn_kernel<_Float16, true, MODE> : paged_attn_kernel<_Float16, false, MODE>;
     return eight ? paged_attn_kernel<__bf16, true, MODE> : paged_attn_kernel<__bf16, false, MODE>;
   };
-  const auto kern = !pl.tiles ? kernel_of(std::integral_constant<PagedMode, kFewRows>())
-                    : !pl.few ? kernel_of(std::integral_constant<PagedMode, kTiles>())
-                              : kernel_of(std::integral_constant<PagedMode, kBoth>());
+  const auto kern = !tile_blocks   ? kernel_of(std::integral_constant<PagedMode, kFewRows>())
+                    : !few_blocks ? kernel_of(std::integral_constant<PagedMode, kTiles>())
+                                  : kernel_of(std::integral_constant<PagedMode, kBoth>());
   hipError_t e = launch(kern, dim3((uint32_t)(few_blocks + tile_blocks)), 256, 0, stream, p);
-  if (e != hipSuccess) return e;
-  const long long few_folds = pl.few_slots() ? pl.few_tiles * Hkv : 0, tile_folds = pl.tile_slots() ? pl.row_tiles * Hkv * (kTileRows / 16) : 0;
-  if (few_folds + tile_folds == 0) return hipSuccess;
-  if (few_folds + tile_folds > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (e != hipSuccess || few_folds + tile_folds == 0) return e;
   p.few_blocks = (int)few_folds;
   return launch(dt == kDtFloat16 ? paged_combine_kernel<_Float16> : paged_combine_kernel<__bf16>, dim3((uint32_t)(few_folds + tile_folds)), 256, 0,
                 stream, p);

@@ -73,7 +73,7 @@ template <typename T, bool NEOX, bool EIGHT> __global__ __launch_bounds__(256) v
       store_device_b128(out + 128, vb);
       continue;
     }
-    if (at.page < 0) continue;
+    if (!at.there(p.batch)) continue;
     char *page = (is_v ? p.v_pages : p.k_pages) + (int64_t)at.page * p.batch.page_stride;
     const int row = h * page_rows + at.row;
     if constexpr (!EIGHT) {
@@ -136,7 +136,7 @@ template <typename T, bool EIGHT> __global__ __launch_bounds__(256) void paged_r
     const bool is_v = r >= p.kv_heads;
     const int h = r - (is_v ? p.kv_heads : 0);
     u32x4_t v = {0u, 0u, 0u, 0u};
-    if (at.page >= 0) {
+    if (at.there(p.batch)) {
       const char *page = (is_v ? p.v_pages : p.k_pages) + (int64_t)at.page * p.batch.page_stride;
       const int row = h * page_rows + at.row;
       if constexpr (EIGHT) {
