@@ -7,8 +7,8 @@
 // a kv head are read for all g heads at once.  Two kinds of workgroups, of four waves each:
 //
 //  * few rows: a sequence with at most 16 rows.  A stream of K and V through the chip: the rows are the 16 columns of mfma 16x16x32, a wave
-//    takes every fourth piece of 32 keys, which it stages in LDS of its own (flash_decode.hip has the layout and why), and keeps its own
-//    running maximum, sum and O; the four are merged at the end.
+//    takes every fourth piece of 32 keys and keeps its own running maximum, sum and O; the four are merged at the end.  K is loaded as
+//    the operand has it, V goes through LDS of the wave's own and is read transposed.
 //  * tiles: 128 rows, 32 to a wave (wave_attn.hpp), over tiles of 64 keys in LDS, two of them, so that a tile is on its way while
 //    the one before it is worked on.
 //
@@ -34,19 +34,22 @@
 namespace llmhip {
 
 constexpr int kFewCols = 16;     // rows of a few-rows workgroup
+constexpr int kFlagBytes = 16;
 constexpr int kFewUnit = 128;    // keys of a unit, 32 to a wave
 constexpr int kTileRows = 128;   // rows of a tile
 constexpr int kTileUnit = 64;    // keys of a unit
 constexpr int kUnitBytes = kTileUnit * kRowBytes;
 constexpr int kWaveStage = 32 * kRowBytes;  // staging of a few-rows wave, for K and for V
-constexpr int kPagedLds = 64 * 1024;
+constexpr int kFewLds = 8 * kWaveStage, kTilesLds = 4 * kUnitBytes;
 
 // One kind of work of a launch
 struct PagedKind {
   float *o, *ml;     // partials [slot][kv head][row][128], and [2]: maximum (times scale and log2 e), sum
+  char *flags;       // [slot][kv head], see few_rows
   int slots;         // room for so many; 0: nothing is split
-  int least;         // units that a split has at least
-  float share;       // kv heads over the workgroups that the keys are dealt to
+  int least;         // units that a part has at least
+  int parts;         // workgroups of a kv head that run at a time
+  int rounds;        // of these, where parts cannot be made to fit one
 };
 struct PagedAttn {
   PagedBatch batch;
@@ -58,8 +61,33 @@ struct PagedAttn {
   int window, sinks;  // window 0: none
   int max_q_len;
   int few_rows;    // sequences of up to so many rows are few-rows ones; 0: none is
-  int few_blocks;  // workgroups of the first kind in a launch of both
+  int tile_blocks;  // workgroups of tiles, the first ones in a launch of both
+  uint64_t number;  // of the launch
 };
+// What the first loads of a workgroup need, in its registers when it starts (common.hpp).
+// a: starts, lengths, page table, q; b: sequences, tokens, max_q_len, few_rows; c: keys_max, heads of a group
+struct PagedEarly {
+  addresses_t a;
+  u32x4_t b;
+  u32x2_t c;
+  explicit PagedEarly(const PagedAttn &p) {
+    a = addresses_t{address(p.batch.q_starts), address(p.batch.kv_lens), address(p.batch.page_table), address(p.q)};
+    b = u32x4_t{(uint32_t)p.batch.batch, (uint32_t)p.batch.tokens, (uint32_t)p.max_q_len, (uint32_t)p.few_rows};
+    c = u32x2_t{(uint32_t)p.batch.keys_max, (uint32_t)p.g};
+  }
+};
+__device__ __forceinline__ void take_early(PagedAttn &p, addresses_t a, u32x4_t b, u32x2_t c) {
+  p.batch.q_starts = at_address<const int>(a[0]);
+  p.batch.kv_lens = at_address<const int>(a[1]);
+  p.batch.page_table = at_address<const int>(a[2]);
+  p.q = at_address<const char>(a[3]);
+  p.batch.batch = b[0];
+  p.batch.tokens = b[1];
+  p.max_q_len = b[2];
+  p.few_rows = b[3];
+  p.batch.keys_max = c[0];
+  p.g = c[1];
+}
 
 __device__ __forceinline__ float bits_to_float(int x) { return __builtin_bit_cast(float, x); }
 __device__ __forceinline__ int float_to_bits(float x) { return __builtin_bit_cast(int, x); }
@@ -121,28 +149,52 @@ template <bool FEW> struct PagedSeqs {
   }
 };
 
-// Dealing keys to workgroups.  The units of all tiles of a kind (each counted like its sequence's last) over the workgroups there are for
-// them make a chunk; a sequence's tiles are split into as many parts as it has chunks.  That is at most one part more to a tile than there
-// are workgroups, and a sequence in parts has at least half a chunk to a part: at most twice as many partials as workgroups.  Whoever needs
-// it works it out by itself, with the same instructions, so all agree; a sequence whose partials find no room is not split.
+// Dealing keys to workgroups.  A sequence's tiles are split into as many parts as it has chunks of units; the chunk is the least for which
+// all parts of all tiles (each counted like its sequence's last) run at a time.  Where there are too many tiles for that, the chunk is that of
+// several rounds.  That is at most a part to a tile more than run in those rounds, and a sequence in parts has at least half a chunk to a
+// part: at most twice as many partials.  Whoever needs it works it out by itself, with the same instructions, so all agree; a
+// sequence whose partials find no room is not split.
 //
 // FOLD: the tile of number w among those that are split.  Else: the part of number w of all; a sequence's last tiles first.
+__device__ __forceinline__ int parts_of(int units, float chunk) {
+  return max((int)__builtin_ceilf((float)units * __builtin_amdgcn_rcpf(chunk) * (1.0f - 0x1p-20f)), 1);  // (a whole number stays one)
+}
+template <typename X> __device__ __forceinline__ X wave_sum(X x) {
+  return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_prefix(x)), 63));
+}
 template <bool FEW, bool FOLD> __device__ __forceinline__ bool find_work(const PagedAttn &p, int w, int lane, PagedTile &t) {
   const PagedKind &kind = FEW ? p.few : p.tiles;
+  PagedSeqs<FEW> s(p, 0, lane);
   float chunk = 0.0f;
   if (kind.slots) {
-    for (int base = 0; base < p.batch.batch; base += 64) {
-      const PagedSeqs<FEW> s(p, base, lane);
-      chunk += bits_to_float(__builtin_amdgcn_readlane(float_to_bits(wave_prefix((float)s.tiles * (float)s.units)), 63));
+    float units = 0.0f;
+    for (int base = 0;;) {
+      units += wave_sum((float)s.tiles * (float)s.units);
+      if ((base += 64) >= p.batch.batch) break;
+      s = PagedSeqs<FEW>(p, base, lane);
     }
-    chunk = fmaxf(chunk * kind.share, (float)kind.least);
+    const float least = (float)kind.least;
+    chunk = fmaxf(units * __builtin_amdgcn_rcpf((float)(kind.parts * kind.rounds)), least);
+    if (p.batch.batch <= 64) {
+      const int tiles = wave_sum(s.tiles);
+      for (int fit = kind.parts, tries = 0; tries < 6 && 2 * fit > kind.parts && tiles <= kind.parts; ++tries) {
+        const float tried = fmaxf(units * __builtin_amdgcn_rcpf((float)fit), least);
+        const int over = wave_sum(s.tiles * parts_of(s.units, tried)) - kind.parts;
+        if (over <= 0) {
+          chunk = tried;
+          break;
+        }
+        fit -= over;
+      }
+    } else {
+      s = PagedSeqs<FEW>(p, 0, lane);
+    }
   }
   int slot = 0;
   for (int base = 0; base < p.batch.batch; base += 64) {
-    const PagedSeqs<FEW> s(p, base, lane);
-    int splits = 1;
-    if (kind.slots) splits = max((int)__builtin_ceilf((float)s.units * __builtin_amdgcn_rcpf(chunk) * (1.0f - 0x1p-20f)), 1);  // (a whole number stays one)
-    int partials = splits > 1 ? s.tiles * splits : 0;
+    if (base > 0) s = PagedSeqs<FEW>(p, base, lane);
+    int splits = kind.slots ? parts_of(s.units, chunk) : 1;
+    const int partials = splits > 1 ? s.tiles * splits : 0;
     const int slots_upto = slot + wave_prefix(partials);
     if (slots_upto > kind.slots) splits = 1;
     const int mine = FOLD ? (splits > 1 ? s.tiles : 0) : s.tiles * splits;
@@ -308,6 +360,9 @@ __device__ __forceinline__ void exact_row(const PagedAttn &p, int b, int kvh, co
 template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const PagedAttn &p, int unit, char *lds) {
   using E = Elem<T>;
   constexpr int kLoads = EIGHT ? 4 : 8;  // of 1 KiB, for 32 rows
+  constexpr int W = cached_row_bytes(EIGHT);
+  constexpr bool kStaged = !EIGHT;
+  constexpr int kAhead = EIGHT ? 2 : 1;  // steps on their way
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, cg = lane >> 4;
   const int item = (int)fast_div(unit, p.Hkv_div), kvh = unit - item * p.Hkv;
   PagedTile t;
@@ -316,6 +371,14 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const
   const PagedKeys keys = keys_seen<kFewUnit>(p, p0, p1, t.len);
   const PagedPart part = part_of(t, keys.units);
 
+  const int iters = part.u1 - part.u0;
+  auto piece = [&](int it) { return keys.base(part.u0 + it, kFewUnit) + 32 * wave; };
+  auto look = [&](int it) {  // 32 steps, two groups each
+    const int i = it + (lane >> 1), u = part.u0 + i;
+    return group_look(p, t.b, kvh, keys.base(u, kFewUnit) + 32 * wave + 16 * (lane & 1), i < iters ? keys.limit(u) : 0);
+  };
+  GroupLook later = look(0);  // (before Q: loads come back in order)
+
   const bool col_valid = col < t.rows;
   const int c_tok = col_valid ? (int)fast_div(col, p.g_div) : 0, c_head = kvh * p.g + (col_valid ? col - c_tok * p.g : 0);
   const int c_pos = p0 + c_tok;
@@ -323,47 +386,53 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) qf[kk] = u32x4_t{0u, 0u, 0u, 0u};
   if (col_valid) {
-    const char *qp = p.q + ((size_t)(t.start + c_tok) * p.H + c_head) * kRowBytes + cg * 16;
+    // Dims of a lane's fragment kk: 32 kk + 8 cg .. + 7; in 8 bits, where its 16 bytes of K are 16 dims, 64 (kk / 2) + 16 cg + 8 (kk % 2)
+    const char *qp = p.q + ((size_t)(t.start + c_tok) * p.H + c_head) * kRowBytes + cg * (EIGHT && !kStaged ? 32 : 16);
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) qf[kk] = global_load_b128(qp + kk * 64);
+    for (int kk = 0; kk < 4; ++kk) qf[kk] = global_load_b128(qp + (EIGHT && !kStaged ? 128 * (kk >> 1) + 16 * (kk & 1) : 64 * kk));
   }
 
   char *vl = lds + wave * kWaveStage, *kl = lds + (4 + wave) * kWaveStage;
-  u32x4_t kn[kLoads], vn[kLoads];
-  int exps = 0;  // 8 bits: of K's 32 rows in the lower lanes, of V's in the upper ones
-  const int iters = part.u1 - part.u0;
-  auto piece = [&](int it) { return keys.base(part.u0 + it, kFewUnit) + 32 * wave; };
-  auto look = [&](int it) {  // 32 steps, two groups each
-    const int i = it + (lane >> 1), u = part.u0 + i;
-    return group_look(p, t.b, kvh, keys.base(u, kFewUnit) + 32 * wave + 16 * (lane & 1), i < iters ? keys.limit(u) : 0);
-  };
-  GroupLook later = {-1, 0};
   GroupPlaces places = {0, 0, 0};
   auto group = [&](int it, int half) { return group_at(places, (it & 31) * 2 + half); };
-  auto issue = [&](const char *pool, u32x4_t (&to)[kLoads], const Group (&g)[2]) {
+  // A step's 32 keys on their way: two steps are
+  struct Step {
+    Group g[2];
+    u32x4_t k[kLoads], v[kLoads];
+    uint8_t k_exps[2], v_exps[2];  // 8 bits: bytes of rows col (K) and lane % 16 (V) of either group
+  };
+  auto fetch = [&](Step &s, int it) {
+    if (it >= iters) return;
+    if ((it & 31) == 0 && it > 0) {
+      places = group_places<EIGHT>(p, later);
+      later = look(it + 32);
+    }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const __amdgpu_buffer_rsrc_t r = group_buffer<EIGHT>(pool, g[half]);
+      s.g[half] = group_at(places, (it & 31) * 2 + half);
+      const __amdgpu_buffer_rsrc_t r = group_buffer<EIGHT>(p.k, s.g[half]);
 #pragma unroll
-      for (int i = 0; i < kLoads / 2; ++i) to[half * (kLoads / 2) + i] = stream_load(r, i * 1024 + lane * 16);
+      for (int i = 0; i < kLoads / 2; ++i) s.k[half * (kLoads / 2) + i] = stream_load(r, kStaged ? i * 1024 + lane * 16 : col * W + cg * 16 + i * 64);
+      if constexpr (EIGHT) s.k_exps[half] = __builtin_amdgcn_raw_buffer_load_b8(byte_buffer(group_exponents(p, p.k, s.g[half]), s.g[half].have()), col, 0, 0);
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const __amdgpu_buffer_rsrc_t r = group_buffer<EIGHT>(p.v, s.g[half]);
+#pragma unroll
+      for (int i = 0; i < kLoads / 2; ++i) s.v[half * (kLoads / 2) + i] = stream_load(r, i * 1024 + lane * 16);
+      if constexpr (EIGHT) s.v_exps[half] = __builtin_amdgcn_raw_buffer_load_b8(byte_buffer(group_exponents(p, p.v, s.g[half]), s.g[half].have()), col, 0, 0);
     }
   };
-  auto issue_exponents = [&](const Group (&g)[2]) {
-    if constexpr (EIGHT) {
-      const char *pool = lane < 32 ? p.k : p.v;
-      const bool second = lane & 16;
-      exps = 127;
-      if ((lane & 15) < (second ? g[1].have() : g[0].have()))
-        exps = *((second ? group_exponents(p, pool, g[1]) : group_exponents(p, pool, g[0])) + (lane & 15));
-    }
-  };
-  // Row of a piece that load i of this lane belongs to, and where its 16 bytes (or what 16 e4m3 become) go
-  auto stage = [&](char *to, const u32x4_t (&from)[kLoads], int which, auto place) {
+  f32x4_t o[8];
+#pragma unroll
+  for (int d = 0; d < 8; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m_run = -INFINITY, l_run = 0.0f;
+  auto stage = [&](const u32x4_t (&from)[kLoads], const uint8_t (&exps)[2], char *to, auto place) {
     if constexpr (EIGHT) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int row = 8 * i + (lane >> 3), granule = 2 * (lane & 7);
-        const float scale = power_of_two(__builtin_amdgcn_ds_bpermute(4 * (row + 32 * which), exps));
+        const float scale = power_of_two(__builtin_amdgcn_ds_bpermute(4 * (row & 15), exps[i >> 1]));
         lds_write_b128(to, place(row, granule), widen8<T>(from[i][0], from[i][1], scale));
         lds_write_b128(to, place(row, granule + 1), widen8<T>(from[i][2], from[i][3], scale));
       }
@@ -372,59 +441,46 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const
       for (int i = 0; i < kLoads; ++i) lds_write_b128(to, place(4 * i + cg, col), from[i]);
     }
   };
-
-  f32x4_t o[8];
-#pragma unroll
-  for (int d = 0; d < 8; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m_run = -INFINITY, l_run = 0.0f;
-  Group now[2];
-  if (iters > 0) {
-    later = look(0);
-    places = group_places<EIGHT>(p, later);
-    later = look(32);
-    now[0] = group(0, 0);
-    now[1] = group(0, 1);
-    issue(p.k, kn, now);
-    issue(p.v, vn, now);
-    issue_exponents(now);
-  }
-  for (int it = 0; it < iters; ++it) {
+  auto step = [&](Step &in, int it) {
     const int base = piece(it), limit = keys.limit(part.u0 + it);
-    const bool whole = now[0].have() == kPageGroup && now[1].have() == kPageGroup;
-    const bool any = now[0].have() + now[1].have() > 0;
-    if (any) {
+    const bool whole = in.g[0].have() == kPageGroup && in.g[1].have() == kPageGroup;
+    const bool there[2] = {in.g[0].have() > 0, in.g[1].have() > 0};
+    if constexpr (kStaged) {
       __builtin_amdgcn_wave_barrier();
-      stage(kl, kn, 0, [](int row, int granule) { return k_swizzle_off(row, granule); });
-      stage(vl, vn, 1, [](int row, int granule) { return v_swizzle32_off(row, granule); });
+      stage(in.k, in.k_exps, kl, [](int row, int granule) { return k_swizzle_off(row, granule); });
       __builtin_amdgcn_wave_barrier();
     }
-    const bool there[2] = {now[0].have() > 0, now[1].have() > 0};
-    if (it + 1 < iters) {
-      if (((it + 1) & 31) == 0) {
-        places = group_places<EIGHT>(p, later);
-        later = look(it + 33);
-      }
-      now[0] = group(it + 1, 0);
-      now[1] = group(it + 1, 1);
-      issue(p.k, kn, now);
-      issue(p.v, vn, now);
-      issue_exponents(now);
-    }
-    if (!any) continue;
+    // ---- S^T = K Q^T ----
     f32x4_t s[2];
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
       s[blk] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) s[blk] = E::mfma16(lds_read_b128(kl, k_swizzle_off(blk * 16 + col, 4 * kk + cg)), qf[kk], s[blk]);
+      for (int kk = 0; kk < 4; ++kk) {
+        if constexpr (kStaged) {
+          s[blk] = E::mfma16(lds_read_b128(kl, k_swizzle_off(blk * 16 + col, 4 * kk + cg)), qf[kk], s[blk]);
+        } else if constexpr (EIGHT) {
+          const u32x4_t from = in.k[2 * blk + (kk >> 1)];
+          s[blk] = E::mfma16(widen8<T>(from[2 * (kk & 1)], from[2 * (kk & 1) + 1], power_of_two(in.k_exps[blk])), qf[kk], s[blk]);
+        } else {
+          s[blk] = E::mfma16(in.k[4 * blk + kk], qf[kk], s[blk]);
+        }
+      }
     }
+    __builtin_amdgcn_wave_barrier();
+    stage(in.v, in.v_exps, vl, [](int row, int granule) { return v_swizzle32_off(row, granule); });
+    __builtin_amdgcn_wave_barrier();
+    fetch(in, it + kAhead);
+    if (!there[0] && !there[1]) return;
     if (!whole || base + 31 > p0 || (p.window > 0 && base <= p1 - p.window && base + 31 >= p.sinks)) {
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = base + blk * 16 + 4 * cg + i;
-          if (!there[blk] || key >= limit || !sees(p, c_pos, key)) s[blk][i] = -INFINITY;
+          const bool hidden = (int)!there[blk] | (int)(key >= limit) | (int)(key > c_pos) |
+                              ((int)(p.window > 0) & (int)(key <= c_pos - p.window) & (int)(key >= p.sinks));
+          s[blk][i] = hidden ? -INFINITY : s[blk][i];
         }
     }
     float mloc = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
@@ -448,6 +504,7 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const
     // denominator carry the same rounding.
     const u32x4_t pf = {E::pack2(s[0][0], s[0][1]), E::pack2(s[0][2], s[0][3]), E::pack2(s[1][0], s[1][1]), E::pack2(s[1][2], s[1][3])};
     l_run += dot2_ones<T>(pf[3], dot2_ones<T>(pf[2], dot2_ones<T>(pf[1], dot2_ones<T>(pf[0], 0.0f))));
+    // ---- O^T += V^T P^T ----
     const int vr = 4 * cg + (col >> 2), sub = (col & 1) * 8;
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
@@ -455,6 +512,17 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const
       const u32x2_t lo = lds_read_tr16(vl, v_swizzle32_off(vr, gran) + sub);
       const u32x2_t hi = lds_read_tr16(vl, v_swizzle32_off(vr + 16, gran) + sub);
       o[d] = E::mfma16(u32x4_t{lo[0], lo[1], hi[0], hi[1]}, pf, o[d]);
+    }
+  };
+  if (iters > 0) {
+    places = group_places<EIGHT>(p, later);
+    later = look(32);
+    Step a = {}, b = {};
+    fetch(a, 0);
+    if (kAhead > 1) fetch(b, 1);
+    for (int it = 0; it < iters; it += kAhead) {
+      step(a, it);
+      if (kAhead > 1 && it + 1 < iters) step(b, it + 1);
     }
   }
 
@@ -470,46 +538,113 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const
   }
   __syncthreads();
   const int c = tid >> 4, dch = tid & 15;  // 16 lanes to a row, 8 dims each
-  if (c >= t.rows) return;
   float M = -INFINITY, L = 0.0f, acc[8];
-#pragma unroll
-  for (int w = 0; w < 4; ++w) M = fmaxf(M, lml[(w * kFewCols + c) * 2]);
-  const float M_use = M == -INFINITY ? 0.0f : M;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float wt = fast_exp2(lml[(w * kFewCols + c) * 2] - M_use);
-    L += wt * lml[(w * kFewCols + c) * 2 + 1];
-    const float *src = lo_f + (w * kFewCols + c) * kHeadDim;
-    const f32x4_t s0 = *reinterpret_cast<const f32x4_t *>(src + (((2 * dch) ^ c) << 2)), s1 = *reinterpret_cast<const f32x4_t *>(src + (((2 * dch + 1) ^ c) << 2));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      acc[j] += wt * s0[j];
-      acc[4 + j] += wt * s1[j];
-    }
-  }
   const int tok = (int)fast_div(c, p.g_div);
   const size_t row_at = ((size_t)(t.start + tok) * p.H + kvh * p.g + c - tok * p.g) * kRowBytes;
-  float size = 0.0f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) size += __builtin_fabsf(acc[j]);
-  const bool finite = size < INFINITY;
-  if (__builtin_expect(((__builtin_amdgcn_ballot_w64(!finite) >> (lane & 48)) & 0xffff) != 0, 0))
-    exact_row<T, EIGHT, 16, kFewUnit>(p, t.b, kvh, p.q + row_at, p0 + tok, keys, part.u0, part.u1, M, L, acc);
-  if (t.splits == 1) {
+  auto store_row = [&] {
     const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);  // (NaN stays NaN)
     u32x4_t w;
 #pragma unroll
     for (int j = 0; j < 4; ++j) w[j] = E::pack2(acc[2 * j] * inv, acc[2 * j + 1] * inv);
     *reinterpret_cast<u32x4_t *>(p.out + row_at + dch * 16) = w;
-    return;
+  };
+  const int bytes = p.few.slots * p.Hkv * kFewCols;
+  const __amdgpu_buffer_rsrc_t po = byte_buffer(p.few.o, bytes * kHeadDim * 4), pml = byte_buffer(p.few.ml, bytes * 8);
+  auto slot_row = [&](int part_) { return ((t.slot + part_) * p.Hkv + kvh) * kFewCols + c; };
+  if (c < t.rows) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, lml[(w * kFewCols + c) * 2]);
+    const float M_use = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float wt = fast_exp2(lml[(w * kFewCols + c) * 2] - M_use);
+      L += wt * lml[(w * kFewCols + c) * 2 + 1];
+      const float *src = lo_f + (w * kFewCols + c) * kHeadDim;
+      const f32x4_t s0 = *reinterpret_cast<const f32x4_t *>(src + (((2 * dch) ^ c) << 2)), s1 = *reinterpret_cast<const f32x4_t *>(src + (((2 * dch + 1) ^ c) << 2));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        acc[j] += wt * s0[j];
+        acc[4 + j] += wt * s1[j];
+      }
+    }
+    float size = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) size += __builtin_fabsf(acc[j]);
+    const bool finite = size < INFINITY;
+    if (__builtin_expect(((__builtin_amdgcn_ballot_w64(!finite) >> (lane & 48)) & 0xffff) != 0, 0))
+      exact_row<T, EIGHT, 16, kFewUnit>(p, t.b, kvh, p.q + row_at, p0 + tok, keys, part.u0, part.u1, M, L, acc);
+    if (t.splits == 1) {
+      store_row();
+    } else {
+      store_device(po, slot_row(t.split) * 512 + dch * 32, f32x4_t{acc[0], acc[1], acc[2], acc[3]});
+      store_device(po, slot_row(t.split) * 512 + dch * 32 + 16, f32x4_t{acc[4], acc[5], acc[6], acc[7]});
+      if (dch == 0) store_device(pml, slot_row(t.split) * 8, u32x2_t{__builtin_bit_cast(uint32_t, M), __builtin_bit_cast(uint32_t, L)});
+    }
   }
-  const size_t slot = ((size_t)(t.slot + t.split) * p.Hkv + kvh) * kFewCols + c;
-  float *wo = p.few.o + slot * kHeadDim + 8 * dch;
-  *reinterpret_cast<f32x4_t *>(wo) = f32x4_t{acc[0], acc[1], acc[2], acc[3]};
-  *reinterpret_cast<f32x4_t *>(wo + 4) = f32x4_t{acc[4], acc[5], acc[6], acc[7]};
-  if (dch == 0) *reinterpret_cast<float2 *>(p.few.ml + slot * 2) = float2{M, L};
+  if (t.splits == 1) return;
+  // The partials are folded by the workgroup that finds all of them stored.  Each raises its flag once its partial is where all XCDs see it,
+  // and looks at the others' after that: the last one to raise its flag finds all of them up (if two do, both write the same rows).  A
+  // flag is up if it holds the launch's number, whatever the workspace held before; who folds takes them down for a replay.  Nobody waits
+  // for another.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  unsigned *all_up = reinterpret_cast<unsigned *>(lds);
+  const __amdgpu_buffer_rsrc_t pf = byte_buffer(p.few.flags, p.few.slots * p.Hkv * kFlagBytes);
+  auto flag_at = [&](int part_) { return ((t.slot + part_) * p.Hkv + kvh) * kFlagBytes; };
+  if (wave == 0) {
+    const u32x2_t up = {(uint32_t)p.number, (uint32_t)(p.number >> 32)};
+    if (lane == 0) store_device(pf, flag_at(t.split), up);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    bool down = false;
+    for (int i = lane; i < t.splits; i += 64) {
+      const u32x2_t f = load_device2(pf, flag_at(i));
+      down |= f[0] != up[0] || f[1] != up[1];
+    }
+    const bool all = __builtin_amdgcn_ballot_w64(down) == 0;
+    if (lane == 0) *all_up = all;
+  }
+  __syncthreads();
+  if (*all_up == 0) return;
+  for (int i = tid; i < t.splits; i += 256) store_device(pf, flag_at(i), u32x2_t{0u, 0u});
+  if (c >= t.rows) return;
+  M = -INFINITY;
+  L = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
+  constexpr int D = 8;  // on their way at a time
+  for (int s0 = 0; s0 < t.splits; s0 += D) {
+    u32x2_t ml[D];
+    f32x4_t x[D], y[D];
+#pragma unroll
+    for (int j = 0; j < D; ++j) {
+      const int at = slot_row(min(s0 + j, t.splits - 1));
+      ml[j] = load_device2(pml, at * 8);
+      x[j] = load_device(po, at * 512 + dch * 32);
+      y[j] = load_device(po, at * 512 + dch * 32 + 16);
+    }
+    float most = M;
+#pragma unroll
+    for (int j = 0; j < D; ++j) most = fmaxf(most, __builtin_bit_cast(float, (uint32_t)ml[j][0]));
+    const float m_use = most == -INFINITY ? 0.0f : most, before = fast_exp2(M - m_use);
+    M = most;
+    L *= before;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] *= before;
+#pragma unroll
+    for (int j = 0; j < D; ++j) {
+      if (s0 + j >= t.splits) continue;
+      const float wt = fast_exp2(__builtin_bit_cast(float, (uint32_t)ml[j][0]) - m_use);
+      L += wt * __builtin_bit_cast(float, (uint32_t)ml[j][1]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        acc[i] += wt * x[j][i];
+        acc[4 + i] += wt * y[j][i];
+      }
+    }
+  }
+  store_row();
 }
 
 // ---- tiles ----
@@ -539,6 +674,13 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
   const int p0 = before + (int)fast_div(t.row0, p.g_div), p1 = before + (int)fast_div(t.row0 + t.rows - 1, p.g_div);
   const PagedKeys keys = keys_seen<kTileUnit>(p, p0, p1, t.len);
   const PagedPart part = part_of(t, keys.units);
+
+  const int iters = part.u1 - part.u0;
+  auto look = [&](int it) {  // 16 tiles, four groups each
+    const int i = it + (lane >> 2), u = part.u0 + i;
+    return group_look(p, t.b, kvh, keys.base(u, kTileUnit) + 16 * (lane & 3), i < iters ? keys.limit(u) : 0);
+  };
+  GroupLook later = look(0);  // (before Q: loads come back in order)
 
   // this wave's rows, and this lane's
   const int w_rows = min(t.rows - 32 * wave, 32), w_row0 = t.row0 + 32 * wave;  // (none: w_rows <= 0)
@@ -571,12 +713,6 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
   u32x4_t kn[2], vn[2];  // 8 bits: what is on its way to slots of K and V
   int exps = 0;
 
-  const int iters = part.u1 - part.u0;
-  auto look = [&](int it) {  // 16 tiles, four groups each
-    const int i = it + (lane >> 2), u = part.u0 + i;
-    return group_look(p, t.b, kvh, keys.base(u, kTileUnit) + 16 * (lane & 3), i < iters ? keys.limit(u) : 0);
-  };
-  GroupLook later = {-1, 0};
   GroupPlaces places = {0, 0, 0};
   // Where this wave's group of tile `it` is, and which groups of the tile are there at all
   struct Next {
@@ -643,7 +779,6 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
   float scale = kScaleLog2e;
   asm volatile("" : "+s"(scale));
   if (iters > 0) {
-    later = look(0);
     cur = next_of(0);
     nxt = next_of(1);
     after = next_of(2);
@@ -769,28 +904,26 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
 
 enum PagedMode { kFewRows, kTiles, kBoth };
 
-template <typename T, bool EIGHT, PagedMode MODE> __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedAttn p) {
-  __shared__ __attribute__((aligned(16))) char lds[kPagedLds];
+template <typename T, bool EIGHT, PagedMode MODE> __global__ __launch_bounds__(256, 2) void paged_attn_kernel(addresses_t a, u32x4_t b, u32x2_t c, PagedAttn p) {
+  take_early(p, a, b, c);
+  __shared__ __attribute__((aligned(16))) char lds[MODE == kFewRows ? kFewLds : kTilesLds];
   const int unit = blockIdx.x;
-  if (MODE == kFewRows || (MODE == kBoth && unit < p.few_blocks))
-    few_rows<T, EIGHT>(p, unit, lds);
+  if (MODE == kFewRows || (MODE == kBoth && unit >= p.tile_blocks))
+    few_rows<T, EIGHT>(p, unit - (MODE == kBoth ? p.tile_blocks : 0), lds);
   else
-    tile_rows<T, EIGHT>(p, unit - (MODE == kBoth ? p.few_blocks : 0), lds);
+    tile_rows<T, EIGHT>(p, unit, lds);
 }
 
-// Partials of a (tile, kv head), 8 rows to a workgroup, 32 lanes of 4 dims to a row; 8 partials are on their way at a time.
-template <typename T> __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttn p) {
+// Partials of a tile of a kv head, 8 rows to a workgroup, 32 lanes of 4 dims to a row; 8 partials are on their way at a time.
+template <typename T> __global__ __launch_bounds__(256) void paged_combine_kernel(addresses_t a, u32x4_t b, u32x2_t c_, PagedAttn p) {
+  take_early(p, a, b, c_);
   const int tid = threadIdx.x, lane = tid & 63, d4 = (tid & 31) * 4;
-  const bool few = (int)blockIdx.x < p.few_blocks;
-  const int block = few ? blockIdx.x : blockIdx.x - p.few_blocks, slot_rows = few ? kFewCols : kTileRows;
-  const int unit = block / (few ? kFewCols / 8 : kTileRows / 8), c = (block % (few ? kFewCols / 8 : kTileRows / 8)) * 8 + (tid >> 5);
+  const int unit = blockIdx.x / (kTileRows / 8), c = blockIdx.x % (kTileRows / 8) * 8 + (tid >> 5);
   const int item = (int)fast_div(unit, p.Hkv_div), kvh = unit - item * p.Hkv;
   PagedTile t;
-  if (!(few ? find_work<true, true>(p, item, lane, t) : find_work<false, true>(p, item, lane, t))) return;
-  if (c >= t.rows) return;
-  const PagedKind &kind = few ? p.few : p.tiles;
-  const size_t row = ((size_t)t.slot * p.Hkv + kvh) * slot_rows + c, step = (size_t)p.Hkv * slot_rows;
-  const float *po = kind.o + row * kHeadDim + d4, *pml = kind.ml + row * 2;
+  if (!find_work<false, true>(p, item, lane, t) || c >= t.rows) return;
+  const size_t row = ((size_t)t.slot * p.Hkv + kvh) * kTileRows + c, step = (size_t)p.Hkv * kTileRows;
+  const float *po = p.tiles.o + row * kHeadDim + d4, *pml = p.tiles.ml + row * 2;
   float M = -INFINITY, L = 0.0f;
   f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
   constexpr int D = 8;
@@ -829,9 +962,9 @@ template <typename T> __global__ __launch_bounds__(256) void paged_combine_kerne
 struct PagedPlan {
   struct Kind {
     long long tiles, items, slots, rows;  // at most; rows of a partial
-    int least;
-    float share;
-    size_t bytes(int Hkv) const { return (size_t)slots * Hkv * rows * (kHeadDim + 2) * sizeof(float); }
+    int least, parts, rounds;
+    bool flags;
+    size_t bytes(int Hkv) const { return (size_t)slots * Hkv * (rows * (kHeadDim + 2) * sizeof(float) + (flags ? kFlagBytes : 0)); }
     long long folds() const { return slots / 2 < tiles ? slots / 2 : tiles; }  // tiles that are split, at most
   } few, by_tiles;
   size_t bytes(int Hkv) const { return few.bytes(Hkv) + by_tiles.bytes(Hkv); }
@@ -843,21 +976,21 @@ static PagedPlan plan_paged(int tokens, int batch, int max_q_len, int max_kv_len
   // (all sequences have max_q_len tokens, or the tokens do not add up: no few-rows ones)
   if (!tiles || (g <= kFewCols && (long long)batch * max_q_len != tokens)) pl.few.tiles = sequences;
   if (tiles) pl.by_tiles.tiles = (long long)tokens * g / kTileRows + sequences;
-  auto deal = [&](PagedPlan::Kind &kind, int rows, int unit, long long span, long long workgroups, int least) {
+  auto deal = [&](PagedPlan::Kind &kind, int rows, int unit, long long span, long long workgroups, int rounds, int least) {
     kind.rows = rows;
+    kind.flags = rows == kFewCols;
     kind.least = least;
-    kind.share = (float)Hkv / (float)workgroups;
+    kind.parts = Hkv <= workgroups ? (int)(workgroups / Hkv) : 1;
+    kind.rounds = rounds;
     const long long windowed = (long long)window + span + sinks + 2 * kPageGroup, seen = window > 0 && windowed < max_kv_len ? windowed : max_kv_len;
-    const long long each = workgroups / Hkv + 1;
-    // in parts: not if no sequence is longer than a part's least, nor if the tiles of even one that is in parts would be more than workgroups
-    const bool parts = kind.tiles > 0 && (seen + unit - 1) / unit > least;
-    kind.slots = parts ? 2 * each + 2 : 0;
-    const long long most = kind.tiles * ((seen + unit - 1) / unit / least + 1);
+    const long long units = (seen + unit - 1) / unit, all = (long long)kind.parts * rounds + 1 + kind.parts * rounds / 64;
+    kind.slots = kind.tiles > 0 && units > least && Hkv <= workgroups ? 2 * all : 0;
+    const long long most = kind.tiles * (units / least + 1);
     if (kind.slots > most) kind.slots = most;
-    kind.items = kind.tiles + (kind.slots ? each + each / 64 + 1 : 0);
+    kind.items = kind.tiles + (kind.slots ? all : 0);
   };
-  deal(pl.few, kFewCols, kFewUnit, kFewCols, 2 * cus, 2);
-  deal(pl.by_tiles, kTileRows, kTileUnit, kTileRows / g + 1, 2 * cus, 6);
+  deal(pl.few, kFewCols, kFewUnit, kFewCols, cus, 1, 3);
+  deal(pl.by_tiles, kTileRows, kTileUnit, kTileRows / g + 1, 2 * cus, 1, 6);
   return pl;
 }
 
@@ -885,16 +1018,18 @@ hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, cons
   p.few_rows = pl.few.tiles ? kFewCols : 0;
   float *ws = static_cast<float *>(workspace);
   auto kind_of = [&](const PagedPlan::Kind &k) {
-    const PagedKind kind = {ws, ws + (size_t)k.slots * Hkv * k.rows * kHeadDim, (int)k.slots, k.least, k.share};
+    float *const ml = ws + (size_t)k.slots * Hkv * k.rows * kHeadDim;
+    const PagedKind kind = {ws, ml, reinterpret_cast<char *>(ml + (size_t)k.slots * Hkv * k.rows * 2), (int)k.slots, k.least, k.parts, k.rounds};
     if (k.slots) ws += k.bytes(Hkv) / sizeof(float);
     return kind;
   };
   p.few = kind_of(pl.few);
   p.tiles = kind_of(pl.by_tiles);
   const long long few_blocks = pl.few.items * Hkv, tile_blocks = pl.by_tiles.items * Hkv;
-  const long long few_folds = pl.few.folds() * Hkv * (kFewCols / 8), tile_folds = pl.by_tiles.folds() * Hkv * (kTileRows / 8);
-  if (few_blocks + tile_blocks > 0x7fffffffLL || few_folds + tile_folds > 0x7fffffffLL) return hipErrorInvalidValue;
-  p.few_blocks = (int)few_blocks;
+  const long long folds = pl.by_tiles.folds() * Hkv * (kTileRows / 8);
+  if (few_blocks + tile_blocks > 0x7fffffffLL || folds > 0x7fffffffLL) return hipErrorInvalidValue;
+  p.number = pl.few.slots ? launch_number() : 0;
+  p.tile_blocks = (int)tile_blocks;
   auto kernel_of = [&](auto mode) {
     constexpr PagedMode MODE = decltype(mode)::value;
     if (dt == kDtFloat16) return eight ? paged_attn_kernel<_Float16, true, MODE> : paged_attn_kernel<_Float16, false, MODE>;
@@ -903,11 +1038,11 @@ hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, cons
   const auto kern = !tile_blocks   ? kernel_of(std::integral_constant<PagedMode, kFewRows>())
                     : !few_blocks ? kernel_of(std::integral_constant<PagedMode, kTiles>())
                                   : kernel_of(std::integral_constant<PagedMode, kBoth>());
-  hipError_t e = launch(kern, dim3((uint32_t)(few_blocks + tile_blocks)), 256, 0, stream, p);
-  if (e != hipSuccess || few_folds + tile_folds == 0) return e;
-  p.few_blocks = (int)few_folds;
-  return launch(dt == kDtFloat16 ? paged_combine_kernel<_Float16> : paged_combine_kernel<__bf16>, dim3((uint32_t)(few_folds + tile_folds)), 256, 0,
-                stream, p);
+  const PagedEarly early(p);
+  const hipError_t e = launch(kern, dim3((uint32_t)(few_blocks + tile_blocks)), 256, 0, stream, early.a, early.b, early.c, p);
+  if (e != hipSuccess || folds == 0) return e;
+  return launch(dt == kDtFloat16 ? paged_combine_kernel<_Float16> : paged_combine_kernel<__bf16>, dim3((uint32_t)folds), 256, 0, stream, early.a,
+                early.b, early.c, p);
 }
 
 }  // namespace llmhip
