@@ -61,6 +61,31 @@ __device__ __forceinline__ int sequence_of(const PagedBatch &p, int token, int l
   return __builtin_amdgcn_readfirstlane(b);
 }
 
+// Where the cached row of a lane's token is.  first: the wave's first token, no later than any of its lanes' and close to them.
+struct TokenPlace {
+  int pos;   // -1: no sequence's token, or of one that is passed over; below that: before the sequence's first row
+  int page;  // -1: nowhere
+  int row;
+};
+__device__ __forceinline__ TokenPlace token_place(const PagedBatch &p, int first, int token, int lane) {
+  TokenPlace t = {-1, -1, 0};
+  int b = sequence_of(p, first, lane);
+  if (token != first)
+    while (b < p.batch && p.q_starts[b + 1] <= token) ++b;
+  if (b >= p.batch || token >= p.tokens) return t;
+  const int start = p.q_starts[b], end = p.q_starts[b + 1], len = p.kv_lens[b];
+  if (token < start || !sequence_ok(p, start, end, len)) return t;
+  t.pos = len - end + token;
+  if (t.pos < 0) {
+    --t.pos;
+    return t;
+  }
+  const PagePlace at = page_place(p, b, t.pos);
+  t.row = at.row;
+  if (at.there(p)) t.page = at.page;
+  return t;
+}
+
 // ---- the 8-bit form ----
 
 constexpr int kLeastExponent = 64;

@@ -17,6 +17,8 @@
 
 namespace llmhip {
 
+constexpr int kManyTokens = 2048, kReadTokens = 4;
+
 struct PagedAppend {
   PagedBatch batch;
   char *out_q, *k_pages, *v_pages;
@@ -48,6 +50,7 @@ template <typename T> __device__ __forceinline__ void limited8(u32x4_t v, float 
   }
 }
 
+// A workgroup has a token, 8 lanes to a row as in rope_kv_append.hip, 32 rows at a time.  Where the token is is the same to all: scalar work.
 template <typename T, bool NEOX, bool EIGHT> __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend p) {
   const int token = blockIdx.x, tid = threadIdx.x, lane = tid & 63, j = tid & 7;
   const int b = sequence_of(p.batch, token, lane);
@@ -98,6 +101,9 @@ template <typename T, bool NEOX, bool EIGHT> __global__ __launch_bounds__(256) v
 hipError_t launch_paged_append(void *out_q, void *k_pages, void *v_pages, const PagedBatch &batch, const void *freq_cis, const void *in_q,
                                const void *in_k, const void *in_v, int table_rows, int q_heads, int kv_heads, int is_neox, bool eight,
                                int dt, hipStream_t stream) {
+  // A token's rows over several workgroups where there are fewer tokens than CUs (us, one / several: 24 tokens of 40 + 2 x 8 heads in 8
+  // bits 5.35 / 4.8; 4096 of 28 + 2 x 4 18.3 / 19.7).
+  const unsigned spread = batch.tokens < device_compute_units() ? (unsigned)(q_heads + 2 * kv_heads + 31) / 32 : 1u;
   const PagedAppend p = {batch,
                          static_cast<char *>(out_q),
                          static_cast<char *>(k_pages),
@@ -114,7 +120,7 @@ hipError_t launch_paged_append(void *out_q, void *k_pages, void *v_pages, const 
     if (eight) return is_neox ? paged_append_kernel<T, true, true> : paged_append_kernel<T, false, true>;
     return is_neox ? paged_append_kernel<T, true, false> : paged_append_kernel<T, false, false>;
   };
-  return launch(dt == kDtFloat16 ? kernel_of(_Float16()) : kernel_of(__bf16()), dim3(batch.tokens), 256, 0, stream, p);
+  return launch(dt == kDtFloat16 ? kernel_of(_Float16()) : kernel_of(__bf16()), dim3(batch.tokens, spread), 256, 0, stream, p);
 }
 
 struct PagedRead {
@@ -124,29 +130,40 @@ struct PagedRead {
   int kv_heads;
 };
 
-template <typename T, bool EIGHT> __global__ __launch_bounds__(256) void paged_read_kernel(PagedRead p) {
-  const int token = blockIdx.x, tid = threadIdx.x, lane = tid & 63, j = tid & 15;
-  const int b = sequence_of(p.batch, token, lane);
-  if (b >= p.batch.batch) return;
-  const int first = p.batch.q_starts[b], end = p.batch.q_starts[b + 1], len = p.batch.kv_lens[b];
-  if (token < first || !sequence_ok(p.batch, first, end, len)) return;
-  const PagePlace at = page_place(p.batch, b, len - end + token);
+// A workgroup has TOKENS tokens; 16 lanes to a row, 16 rows of a token at a time.  All loads of a turn go out before the first is used.
+template <typename T, bool EIGHT, int TOKENS> __global__ __launch_bounds__(256) void paged_read_kernel(PagedRead p) {
+  const int token0 = blockIdx.x * TOKENS, tid = threadIdx.x, lane = tid & 63, j = tid & 15;
+  // (one token to a lane, the first TOKENS lanes)
+  const TokenPlace places = token_place(p.batch, token0, token0 + min(lane, TOKENS - 1), lane);
   const int page_rows = (int)p.batch.page_size.d;
   for (int r = tid >> 4; r < 2 * p.kv_heads; r += 16) {
     const bool is_v = r >= p.kv_heads;
     const int h = r - (is_v ? p.kv_heads : 0);
-    u32x4_t v = {0u, 0u, 0u, 0u};
-    if (at.there(p.batch)) {
-      const char *page = (is_v ? p.v_pages : p.k_pages) + (int64_t)at.page * p.batch.page_stride;
-      const int row = h * page_rows + at.row;
-      if constexpr (EIGHT) {
-        const u32x2_t w = *reinterpret_cast<const u32x2_t *>(page + (size_t)row * kHeadDim + j * 8);
-        v = widen8<T>(w[0], w[1], power_of_two((uint8_t)page[(size_t)p.kv_heads * page_rows * kHeadDim + row]));
-      } else {
-        v = global_load_b128(page + (size_t)row * kRowBytes + j * 16);
-      }
+    const char *pool = is_v ? p.v_pages : p.k_pages;
+    using Raw = std::conditional_t<EIGHT, u32x2_t, u32x4_t>;
+    Raw v[TOKENS];
+    int byte[TOKENS];
+#pragma unroll
+    for (int i = 0; i < TOKENS; ++i) {
+      const int at_page = __builtin_amdgcn_readlane(places.page, i), row = h * page_rows + __builtin_amdgcn_readlane(places.row, i);
+      v[i] = Raw{};
+      byte[i] = 127;
+      if (at_page < 0) continue;
+      const char *page = pool + (int64_t)at_page * p.batch.page_stride;
+      v[i] = __builtin_nontemporal_load(reinterpret_cast<const Raw *>(page + (size_t)row * cached_row_bytes(EIGHT) + j * sizeof(Raw)));
+      if (EIGHT) byte[i] = (uint8_t)page[(size_t)p.kv_heads * page_rows * kHeadDim + row];
     }
-    *reinterpret_cast<u32x4_t *>((is_v ? p.out_v : p.out_k) + ((size_t)token * p.kv_heads + h) * kRowBytes + j * 16) = v;
+    char *out = (is_v ? p.out_v : p.out_k) + ((size_t)token0 * p.kv_heads + h) * kRowBytes + j * 16;
+#pragma unroll
+    for (int i = 0; i < TOKENS; ++i) {
+      if (__builtin_amdgcn_readlane(places.pos, i) == -1) continue;
+      u32x4_t x;
+      if constexpr (EIGHT)
+        x = widen8<T>(v[i][0], v[i][1], power_of_two(byte[i]));
+      else
+        x = v[i];
+      __builtin_nontemporal_store(x, reinterpret_cast<u32x4_t *>(out + (size_t)i * p.kv_heads * kRowBytes));
+    }
   }
 }
 
@@ -158,8 +175,16 @@ hipError_t launch_paged_read(void *out_k, void *out_v, const void *k_pages, cons
                        static_cast<const char *>(k_pages),
                        static_cast<const char *>(v_pages),
                        kv_heads};
-  auto kernel_of = [&](auto t) { return eight ? paged_read_kernel<decltype(t), true> : paged_read_kernel<decltype(t), false>; };
-  return launch(dt == kDtFloat16 ? kernel_of(_Float16()) : kernel_of(__bf16()), dim3(batch.tokens), 256, 0, stream, p);
+  auto kernel_of = [&](auto t, auto tokens) {
+    constexpr int N = decltype(tokens)::value;
+    return eight ? paged_read_kernel<decltype(t), true, N> : paged_read_kernel<decltype(t), false, N>;
+  };
+  const bool many = batch.tokens >= kManyTokens;
+  const std::integral_constant<int, 1> one;
+  const std::integral_constant<int, kReadTokens> some;
+  const auto kern = dt == kDtFloat16 ? (many ? kernel_of(_Float16(), some) : kernel_of(_Float16(), one))
+                                     : (many ? kernel_of(__bf16(), some) : kernel_of(__bf16(), one));
+  return launch(kern, dim3((batch.tokens + (many ? kReadTokens - 1 : 0)) / (many ? kReadTokens : 1)), 256, 0, stream, p);
 }
 
 }  // namespace llmhip
