@@ -162,7 +162,31 @@ __device__ __forceinline__ int parts_of(int units, float chunk) {
 template <typename X> __device__ __forceinline__ X wave_sum(X x) {
   return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_prefix(x)), 63));
 }
+// One sequence by itself: the same in scalar registers, a third of the instructions (which is what workgroups of few tiles
+// wait for: chunk of 200 past 16001, FIGURES).
+template <bool FEW, bool FOLD> __device__ __forceinline__ bool find_alone(const PagedAttn &p, int w, PagedTile &t) {
+  const PagedKind &kind = FEW ? p.few : p.tiles;
+  const int start = p.batch.q_starts[0], end = p.batch.q_starts[1], len = p.batch.kv_lens[0];
+  if (!sequence_ok(p.batch, start, end, len) || end <= start || end - start > p.max_q_len) return false;
+  const int m = end - start, rows = m * p.g;
+  if (FEW != (rows <= p.few_rows)) return false;
+  const int tiles = FEW ? 1 : (rows + kTileRows - 1) / kTileRows, first = FEW ? 0 : (int)fast_div((tiles - 1) * kTileRows, p.g_div);
+  int splits = 1;
+  if (kind.slots && tiles <= kind.parts / 2) {
+    const int units = keys_seen<FEW ? kFewUnit : kTileUnit>(p, len - m + first, len - 1, len).units;
+    splits = max(min(kind.parts / tiles, units / kind.least), 1);
+    if (splits > 1 && tiles * splits > kind.slots) splits = 1;
+  }
+  if (FOLD && splits == 1) return false;
+  const int tile = FOLD || splits == 1 ? w : w / splits;
+  if (tile >= tiles) return false;
+  t = PagedTile{0, start, m, len, FEW ? 0 : (tiles - 1 - tile) * kTileRows, 0, FOLD ? 0 : w - tile * splits, splits, tile * splits};
+  if (!FOLD && splits == 1) t.split = 0;
+  t.rows = min(rows - t.row0, FEW ? kFewCols : kTileRows);
+  return true;
+}
 template <bool FEW, bool FOLD> __device__ __forceinline__ bool find_work(const PagedAttn &p, int w, int lane, PagedTile &t) {
+  if (p.batch.batch == 1) return find_alone<FEW, FOLD>(p, w, t);
   const PagedKind &kind = FEW ? p.few : p.tiles;
   PagedSeqs<FEW> s(p, 0, lane);
   float chunk = 0.0f;
@@ -379,17 +403,15 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const
   };
   GroupLook later = look(0);  // (before Q: loads come back in order)
 
-  const bool col_valid = col < t.rows;
-  const int c_tok = col_valid ? (int)fast_div(col, p.g_div) : 0, c_head = kvh * p.g + (col_valid ? col - c_tok * p.g : 0);
-  const int c_pos = p0 + c_tok;
+  // Columns past the rows have the last row once more.  (Without a branch: the compiler would not know how many loads came after the page
+  // table's, and wait for Q where it needs that one only.)
+  const int c_row = min(col, t.rows - 1), c_tok = (int)fast_div(c_row, p.g_div), c_pos = p0 + c_tok;
   u32x4_t qf[4];
-#pragma unroll
-  for (int kk = 0; kk < 4; ++kk) qf[kk] = u32x4_t{0u, 0u, 0u, 0u};
-  if (col_valid) {
+  {
     // Dims of a lane's fragment kk: 32 kk + 8 cg .. + 7; in 8 bits, where its 16 bytes of K are 16 dims, 64 (kk / 2) + 16 cg + 8 (kk % 2)
-    const char *qp = p.q + ((size_t)(t.start + c_tok) * p.H + c_head) * kRowBytes + cg * (EIGHT && !kStaged ? 32 : 16);
+    const char *qp = p.q + ((size_t)(t.start + c_tok) * p.H + kvh * p.g + c_row - c_tok * p.g) * kRowBytes + cg * (kStaged ? 16 : 32);
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) qf[kk] = global_load_b128(qp + (EIGHT && !kStaged ? 128 * (kk >> 1) + 16 * (kk & 1) : 64 * kk));
+    for (int kk = 0; kk < 4; ++kk) qf[kk] = global_load_b128(qp + (kStaged ? 64 * kk : 128 * (kk >> 1) + 16 * (kk & 1)));
   }
 
   char *vl = lds + wave * kWaveStage, *kl = lds + (4 + wave) * kWaveStage;
@@ -692,11 +714,10 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
     tok = (int)fast_div(w_row0 + r, p.g_div);
     return ((size_t)(t.start + tok) * p.H + kvh * p.g + w_row0 + r - tok * p.g) * kRowBytes;
   };
-  int my_tok = 0;
-#pragma unroll
-  for (int kk = 0; kk < 8; ++kk) w.qf[kk] = u32x4_t{0u, 0u, 0u, 0u};
-  if (w.l32 < w_rows) {
-    const char *qp = p.q + place_of(w.l32, my_tok) + w.hh * 16;
+  int my_tok;
+  {
+    // (rows past the last are that one once more; without a branch, as in few_rows)
+    const char *qp = p.q + place_of(min(w.l32, t.rows - 1 - 32 * wave), my_tok) + w.hh * 16;
 #pragma unroll
     for (int kk = 0; kk < 8; ++kk) w.qf[kk] = global_load_b128(qp + kk * 32);
   }
