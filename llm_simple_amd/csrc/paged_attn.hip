@@ -131,11 +131,13 @@ template <typename X> __device__ __forceinline__ X wave_prefix(X x) {
 // the first part's partial.
 struct PagedTile {
   int b, start, m, len, row0, rows, split, splits, slot;
+  int u0 = 0, u1 = -1;  // a run's part: these units (else u1 < 0, see part_of)
 };
 
 // The sequences of one kind, 64 at a time, a lane each.
 template <bool FEW> struct PagedSeqs {
   int start, m, len, tiles, units;  // units: of the last tile, which sees most
+  PagedSeqs() = default;
   __device__ __forceinline__ PagedSeqs(const PagedAttn &p, int base, int lane) {
     const int i = min(base + lane, p.batch.batch - 1), end = p.batch.q_starts[i + 1];
     start = p.batch.q_starts[i];
@@ -185,7 +187,47 @@ template <bool FEW, bool FOLD> __device__ __forceinline__ bool find_alone(const 
   t.rows = min(rows - t.row0, FEW ? kFewCols : kTileRows);
   return true;
 }
-template <bool FEW, bool FOLD> __device__ __forceinline__ bool find_work(const PagedAttn &p, int w, int lane, PagedTile &t) {
+// Where sequences' lengths leave the greatest chunk well above an equal share, or more parts than run at a time, few-rows workgroups take runs of the units of all sequences
+// one after the other, equal to a unit; a run may end one sequence and begin another, and then costs the start of another.  (us, parts /
+// runs: 48 sequences of up to 16384 keys of 4 kv heads, 48 units to a run, 16 bits 167 / 145, 8 bits 107 / 85; 24 of up to 8192 of 8, 24 units, 76.7 /
+// 72.2 and 52.4 / 51.4; with a window of 4096, 20 units, 61.2 / 67.0; 64 of up to 2048 of 2, 4 units, 19.9 / 23.2.)  A kernel of its own, for
+// bounds that allow runs: the loop over sequences costs a call of 7 us 0.6.
+constexpr int kRunUnits = 24;
+struct FewRuns {
+  PagedSeqs<true> s;
+  int units, upto, slot;  // of a lane's sequence: units, those up to its end, its first partial's slot
+  int total, runs, w, at, end;
+  __device__ __forceinline__ int run_of(int unit) const { return (int)(((uint32_t)(unit + 1) * (uint32_t)runs - 1) / (uint32_t)total); }
+  // False: they are not to be taken in runs.
+  __device__ __forceinline__ bool begin(const PagedAttn &p, int run, int lane) {
+    units = s.tiles ? max(s.units, 1) : 0;
+    upto = wave_prefix(units);
+    total = __builtin_amdgcn_readlane(upto, 63);
+    if (total > 1 << 22) return false;  // (32-bit products)
+    runs = max(min(p.few.parts, total / p.few.least), 1);
+    const int partials = units ? run_of(upto - 1) - run_of(upto - units) + 1 : 0, kept = partials > 1 ? partials : 0, slots_upto = wave_prefix(kept);
+    slot = slots_upto - kept;
+    if (__builtin_amdgcn_readlane(slots_upto, 63) > p.few.slots) return false;
+    w = run;
+    at = (int)((uint32_t)w * (uint32_t)total / (uint32_t)runs);
+    end = w < runs ? (int)((uint32_t)(w + 1) * (uint32_t)total / (uint32_t)runs) : at;
+    return true;
+  }
+  // The next sequence of the run
+  __device__ __forceinline__ bool next(const PagedAttn &p, PagedTile &t) {
+    if (at >= end) return false;
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > at));
+    auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+    const int last = of(upto), first = last - of(units), run0 = run_of(first);
+    t = PagedTile{l, of(s.start), of(s.m), of(s.len), 0, 0, w - run0, run_of(last - 1) - run0 + 1, of(slot), at - first, min(end, last) - first};
+    t.rows = min(t.m * p.g, kFewCols);
+    at = last;
+    return true;
+  }
+};
+// runs: few rows, where it is taken (`in_runs` then says so, and t is not set).
+template <bool FEW, bool FOLD>
+__device__ __forceinline__ bool find_work(const PagedAttn &p, int w, int lane, PagedTile &t, FewRuns *runs = nullptr, bool *in_runs = nullptr) {
   if (p.batch.batch == 1) return find_alone<FEW, FOLD>(p, w, t);
   const PagedKind &kind = FEW ? p.few : p.tiles;
   PagedSeqs<FEW> s(p, 0, lane);
@@ -201,14 +243,25 @@ template <bool FEW, bool FOLD> __device__ __forceinline__ bool find_work(const P
     chunk = fmaxf(units * __builtin_amdgcn_rcpf((float)(kind.parts * kind.rounds)), least);
     if (p.batch.batch <= 64) {
       const int tiles = wave_sum(s.tiles);
+      [[maybe_unused]] bool even = false;
       for (int fit = kind.parts, tries = 0; tries < 6 && 2 * fit > kind.parts && tiles <= kind.parts; ++tries) {
         const float tried = fmaxf(units * __builtin_amdgcn_rcpf((float)fit), least);
         const int over = wave_sum(s.tiles * parts_of(s.units, tried)) - kind.parts;
         if (over <= 0) {
           chunk = tried;
+          even = chunk * (float)kind.parts <= 1.2f * units;
           break;
         }
         fit -= over;
+      }
+      if constexpr (FEW) {
+        if (runs && !even && units >= (float)(kRunUnits * kind.parts)) {
+          runs->s = s;
+          if (runs->begin(p, w, lane)) {
+            *in_runs = true;
+            return true;
+          }
+        }
       }
     } else {
       s = PagedSeqs<FEW>(p, 0, lane);
@@ -251,6 +304,7 @@ struct PagedPart {
   int u0, u1;
 };
 __device__ __forceinline__ PagedPart part_of(const PagedTile &t, int units) {
+  if (t.u1 >= 0) return PagedPart{min(t.u0, units), min(t.u1, units)};
   if (t.splits == 1) return PagedPart{0, units};
   const int each = (units + t.splits - 1) / t.splits, u0 = min(t.split * each, units);
   return PagedPart{u0, min(u0 + each, units)};
@@ -381,16 +435,13 @@ __device__ __forceinline__ void exact_row(const PagedAttn &p, int b, int kvh, co
 
 // ---- few rows ----
 
-template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const PagedAttn &p, int unit, char *lds) {
+template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows_of(const PagedAttn &p, const PagedTile &t, int kvh, char *lds) {
   using E = Elem<T>;
   constexpr int kLoads = EIGHT ? 4 : 8;  // of 1 KiB, for 32 rows
   constexpr int W = cached_row_bytes(EIGHT);
   constexpr bool kStaged = !EIGHT;
   constexpr int kAhead = EIGHT ? 2 : 1;  // steps on their way
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, cg = lane >> 4;
-  const int item = (int)fast_div(unit, p.Hkv_div), kvh = unit - item * p.Hkv;
-  PagedTile t;
-  if (!find_work<true, false>(p, item, lane, t)) return;
   const int p0 = t.len - t.m, p1 = t.len - 1;
   const PagedKeys keys = keys_seen<kFewUnit>(p, p0, p1, t.len);
   const PagedPart part = part_of(t, keys.units);
@@ -669,6 +720,22 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows(const
   store_row();
 }
 
+template <typename T, bool EIGHT, bool RUNS> __device__ __forceinline__ void few_rows(const PagedAttn &p, int unit, char *lds) {
+  const int lane = threadIdx.x & 63, item = (int)fast_div(unit, p.Hkv_div), kvh = unit - item * p.Hkv;
+  PagedTile t;
+  if constexpr (RUNS) {
+    FewRuns runs;
+    bool in_runs = false;
+    if (!find_work<true, false>(p, item, lane, t, &runs, &in_runs) || (in_runs && !runs.next(p, t))) return;
+    for (;;) {
+      few_rows_of<T, EIGHT>(p, t, kvh, lds);
+      if (!in_runs || !runs.next(p, t)) return;
+      __syncthreads();  // (the merge still reads what the next one stages in)
+    }
+  } else {
+    if (find_work<true, false>(p, item, lane, t)) few_rows_of<T, EIGHT>(p, t, kvh, lds);
+  }
+}
 // ---- tiles ----
 
 // 16 rows of a group into LDS, four times 1 KiB, lane by lane: the instruction's offset moves both addresses.  Inline: the compiler would
@@ -923,14 +990,14 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
   }
 }
 
-enum PagedMode { kFewRows, kTiles, kBoth };
+enum PagedMode { kFewRows, kFewRuns, kTiles, kBoth };
 
 template <typename T, bool EIGHT, PagedMode MODE> __global__ __launch_bounds__(256, 2) void paged_attn_kernel(addresses_t a, u32x4_t b, u32x2_t c, PagedAttn p) {
   take_early(p, a, b, c);
-  __shared__ __attribute__((aligned(16))) char lds[MODE == kFewRows ? kFewLds : kTilesLds];
+  __shared__ __attribute__((aligned(16))) char lds[MODE == kFewRows || MODE == kFewRuns ? kFewLds : kTilesLds];
   const int unit = blockIdx.x;
-  if (MODE == kFewRows || (MODE == kBoth && unit >= p.tile_blocks))
-    few_rows<T, EIGHT>(p, unit - (MODE == kBoth ? p.tile_blocks : 0), lds);
+  if (MODE == kFewRows || MODE == kFewRuns || (MODE == kBoth && unit >= p.tile_blocks))
+    few_rows<T, EIGHT, MODE == kFewRuns>(p, unit - (MODE == kBoth ? p.tile_blocks : 0), lds);
   else
     tile_rows<T, EIGHT>(p, unit, lds);
 }
@@ -988,6 +1055,7 @@ struct PagedPlan {
     size_t bytes(int Hkv) const { return (size_t)slots * Hkv * (rows * (kHeadDim + 2) * sizeof(float) + (flags ? kFlagBytes : 0)); }
     long long folds() const { return slots / 2 < tiles ? slots / 2 : tiles; }  // tiles that are split, at most
   } few, by_tiles;
+  bool runs;  // may be taken
   size_t bytes(int Hkv) const { return few.bytes(Hkv) + by_tiles.bytes(Hkv); }
 };
 static PagedPlan plan_paged(int tokens, int batch, int max_q_len, int max_kv_len, int window, int sinks, int g, int Hkv) {
@@ -1009,8 +1077,10 @@ static PagedPlan plan_paged(int tokens, int batch, int max_q_len, int max_kv_len
     const long long most = kind.tiles * (units / least + 1);
     if (kind.slots > most) kind.slots = most;
     kind.items = kind.tiles + (kind.slots ? all : 0);
+    return units;
   };
-  deal(pl.few, kFewCols, kFewUnit, kFewCols, cus, 1, 3);
+  const long long units = deal(pl.few, kFewCols, kFewUnit, kFewCols, cus, 1, 3);
+  pl.runs = batch > 1 && batch <= 64 && pl.few.slots > 0 && pl.few.tiles * units >= (long long)kRunUnits * pl.few.parts;
   deal(pl.by_tiles, kTileRows, kTileUnit, kTileRows / g + 1, 2 * cus, 1, 6);
   return pl;
 }
@@ -1056,7 +1126,8 @@ hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, cons
     if (dt == kDtFloat16) return eight ? paged_attn_kernel<_Float16, true, MODE> : paged_attn_kernel<_Float16, false, MODE>;
     return eight ? paged_attn_kernel<__bf16, true, MODE> : paged_attn_kernel<__bf16, false, MODE>;
   };
-  const auto kern = !tile_blocks   ? kernel_of(std::integral_constant<PagedMode, kFewRows>())
+  const auto kern = !tile_blocks && pl.runs ? kernel_of(std::integral_constant<PagedMode, kFewRuns>())
+                    : !tile_blocks ? kernel_of(std::integral_constant<PagedMode, kFewRows>())
                     : !few_blocks ? kernel_of(std::integral_constant<PagedMode, kTiles>())
                                   : kernel_of(std::integral_constant<PagedMode, kBoth>());
   const PagedEarly early(p);

@@ -34,6 +34,17 @@ def test_decode_in_splits(page_size, eight):
     s.check(out)
 
 
+@pytest.mark.parametrize("kv_heads,lengths,window,sinks,eight", [
+    (256, [(1500, 1), (3, 0), (700, 1), (0, 1), (900, 1)], 0, 0, False), (128, [(2600, 1), (1500, 1), (900, 1), (1, 1), (1300, 1)], 0, 0, True),
+    (128, [(2100, 1), (40, 1), (1900, 1), (2000, 1), (1, 1), (1700, 1)], 1500, 40, False)])
+def test_decode_in_runs(kv_heads, lengths, window, sinks, eight):
+    """Workgroups that end one sequence and begin another: one or two to a kv head, with 24 units of 128 keys or more each."""
+    s = Setup(22, lengths, 1, kv_heads, BF16, eight, 16).to_gpu()
+    out = s.out()
+    s.attend(out, window, sinks)
+    s.check(out, window, sinks)
+
+
 @pytest.mark.parametrize("eight", [False, True])
 @pytest.mark.parametrize("dt", [FP16, BF16])
 @pytest.mark.parametrize("group,kv_heads,page_size", [(1, 2, 16), (7, 1, 48), (3, 2, 32), (17, 1, 16), (40, 1, 64)])
