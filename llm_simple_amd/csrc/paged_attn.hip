@@ -61,7 +61,7 @@ struct PagedAttn {
   int window, sinks;  // window 0: none
   int max_q_len;
   int few_rows;    // sequences of up to so many rows are few-rows ones; 0: none is
-  int tile_blocks;  // workgroups of tiles, the first ones in a launch of both
+  int few_blocks;  // workgroups of few rows, the first ones in a launch of both
   uint64_t number;  // of the launch
 };
 // What the first loads of a workgroup need, in its registers when it starts (common.hpp).
@@ -960,19 +960,43 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
 
   const float l_tot = pair_sum(w.l_run);
   if (t.splits > 1) {
-    if (w.l32 < w_rows) {
-      const size_t slot = ((size_t)(t.slot + t.split) * p.Hkv + kvh) * kTileRows + 32 * wave + w.l32;
-      float *o_row = p.tiles.o + slot * kHeadDim;
+    const size_t slot0 = ((size_t)(t.slot + t.split) * p.Hkv + kvh) * kTileRows + 32 * wave;
+    if (w.l32 < w_rows && w.hh == 0) *reinterpret_cast<float2 *>(p.tiles.ml + (slot0 + w.l32) * 2) = float2{w.m_run * kScaleLog2e, l_tot};
+    if constexpr (EIGHT) {
+      // straight from the accumulators: the registers of this kernel are full (a prompt of 4096 of 28 heads, us: 150, 158 with the way below)
+      if (w.l32 < w_rows) {
+        float *o_row = p.tiles.o + (slot0 + w.l32) * kHeadDim;
 #pragma unroll
-      for (int d = 0; d < 4; ++d)
+        for (int d = 0; d < 4; ++d)
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4)
-          *reinterpret_cast<f32x4_t *>(o_row + 32 * d + 8 * i4 + 4 * w.hh) = f32x4_t{w.o[d][4 * i4], w.o[d][4 * i4 + 1], w.o[d][4 * i4 + 2], w.o[d][4 * i4 + 3]};
-      if (w.hh == 0) *reinterpret_cast<float2 *>(p.tiles.ml + slot * 2) = float2{w.m_run * kScaleLog2e, l_tot};
+          for (int i4 = 0; i4 < 4; ++i4)
+            *reinterpret_cast<f32x4_t *>(o_row + 32 * d + 8 * i4 + 4 * w.hh) = f32x4_t{w.o[d][4 * i4], w.o[d][4 * i4 + 1], w.o[d][4 * i4 + 2], w.o[d][4 * i4 + 3]};
+      }
+      return;
+    }
+    // through 8 KiB of LDS of this wave, half of the dims at a time, so that whole 256-byte pieces leave, past the L2 (us, from the
+    // accumulators / this: 200 tokens past 16001 of 28 + 4 heads 68.1 / 65.3, 20 past 30000 37.8 / 35.8)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int d = 0; d < 2; ++d)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+          const f32x16_t &o = w.o[2 * half + d];
+          const f32x4_t v = {o[4 * i4], o[4 * i4 + 1], o[4 * i4 + 2], o[4 * i4 + 3]};
+          lds_write_b128(mine, k_swizzle_off(w.l32, 8 * d + 2 * i4 + w.hh), __builtin_bit_cast(u32x4_t, v));
+        }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + r4;
+        if (r < w_rows) store_device_b128(p.tiles.o + (slot0 + r) * kHeadDim + 64 * half + c16 * 4, lds_read_b128(mine, k_swizzle_off(r, c16)));
+      }
+      __builtin_amdgcn_wave_barrier();
     }
     return;
   }
-  // through 8 KiB of LDS of this wave, so that whole rows leave
+  // so that whole rows leave
   const float inv = l_tot > 0.0f ? 1.0f / l_tot : (l_tot == 0.0f ? 0.0f : l_tot);  // (NaN stays NaN)
 #pragma unroll
   for (int d = 0; d < 4; ++d)
@@ -996,10 +1020,10 @@ template <typename T, bool EIGHT, PagedMode MODE> __global__ __launch_bounds__(2
   take_early(p, a, b, c);
   __shared__ __attribute__((aligned(16))) char lds[MODE == kFewRows || MODE == kFewRuns ? kFewLds : kTilesLds];
   const int unit = blockIdx.x;
-  if (MODE == kFewRows || MODE == kFewRuns || (MODE == kBoth && unit >= p.tile_blocks))
-    few_rows<T, EIGHT, MODE == kFewRuns>(p, unit - (MODE == kBoth ? p.tile_blocks : 0), lds);
+  if (MODE == kFewRows || MODE == kFewRuns || (MODE == kBoth && unit < p.few_blocks))
+    few_rows<T, EIGHT, MODE == kFewRuns>(p, unit, lds);
   else
-    tile_rows<T, EIGHT>(p, unit, lds);
+    tile_rows<T, EIGHT>(p, unit - (MODE == kBoth ? p.few_blocks : 0), lds);
 }
 
 // Partials of a tile of a kv head, 8 rows to a workgroup, 32 lanes of 4 dims to a row; 8 partials are on their way at a time.
@@ -1120,7 +1144,7 @@ hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, cons
   const long long folds = pl.by_tiles.folds() * Hkv * (kTileRows / 8);
   if (few_blocks + tile_blocks > 0x7fffffffLL || folds > 0x7fffffffLL) return hipErrorInvalidValue;
   p.number = pl.few.slots ? launch_number() : 0;
-  p.tile_blocks = (int)tile_blocks;
+  p.few_blocks = (int)few_blocks;
   auto kernel_of = [&](auto mode) {
     constexpr PagedMode MODE = decltype(mode)::value;
     if (dt == kDtFloat16) return eight ? paged_attn_kernel<_Float16, true, MODE> : paged_attn_kernel<_Float16, false, MODE>;
