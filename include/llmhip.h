@@ -194,9 +194,9 @@ int llmhip_rope_kv_append(void *out_q, void *k_cache, void *v_cache, const void 
  * least llmhip_paged_page_bytes; one allocation may hold both pools, page by page).  A page holds [kv_head_num][page_size] rows of
  * head_dim elements of cache_dt; page_size is a multiple of 16, up to 1024.  cache_dt is dt, or LLMHIP_DT_FLOAT8_E4M3: then a row is
  * 128 e4m3 values times a power of two, 2^(byte - 127), and a page ends with the bytes of its rows, [kv_head_num][page_size].  The
- * byte is the least one, and at least 64, for which the row's largest magnitude is within 448 * 2^(byte - 127).  (Magnitudes above 61440 in fp16 and
- * 1.875 * 2^127 in bf16 count as that; an infinity is stored as NaN and does not count in the byte.)
- * Pools together may be larger than 4 GiB; pages_per_seq * page_size is at most 2^30.
+ * byte is the least one, and at least 64, for which the row's largest magnitude is within 448 * 2^(byte - 127).  (Magnitudes above 61440
+ * in fp16 and 1.875 * 2^127 in bf16 count as that; an infinity is stored as NaN and does not count in the byte.)
+ * Pools may be larger than 4 GiB; pages_per_seq * page_size and tokens are at most 2^30, batch at most 65535.
  *
  * Batch.  All int32, aligned to 4 bytes, in device memory, read when the work runs (a captured graph may be replayed with others):
  *   page_table [batch][pages_per_seq]   pages of a sequence's rows, in order.  A number outside of [0, num_pages) is a page that is
@@ -206,7 +206,8 @@ int llmhip_rope_kv_append(void *out_q, void *k_cache, void *v_cache, const void 
  *   kv_lens [batch]                     rows of the sequence with the new tokens: token t of sequence b is at position
  *                                       kv_lens[b] - q_starts[b + 1] + t, the last one at kv_lens[b] - 1.
  * A sequence whose rows are not all within [0, tokens), or whose length is not within [0, pages_per_seq * page_size], is passed over.
- * No two sequences may write one page, nor have one row.  dense tensors: [tokens][heads][head_dim] of dt. */
+ * Sequences may share pages that nobody writes; no two may append to one row, nor have one row of the dense tensors, [tokens][heads]
+ * [head_dim] of dt. */
 
 /* Bytes of a page of K, or of V; 0 for sizes that the calls below refuse. */
 size_t llmhip_paged_page_bytes(int page_size, int kv_head_num, int head_dim, int cache_dt);

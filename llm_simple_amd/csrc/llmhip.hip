@@ -163,7 +163,7 @@ int paged_common(PagedBatch &b, const int *page_table, const int *q_starts, cons
   if (tokens < 1 || batch < 1 || pages_per_seq < 1 || num_pages < 1 || kv_head_num < 1) return LLMHIP_ERR_INVALID_ARG;
   if (!dtype_ok(dt) || (cache_dt != dt && cache_dt != LLMHIP_DT_FLOAT8_E4M3)) return LLMHIP_ERR_INVALID_ARG;
   if (page_size < 1) return LLMHIP_ERR_INVALID_ARG;
-  if (head_dim != 128 || batch > 65535 || !page_sizes_ok(page_size, kv_head_num, cache_dt)) return LLMHIP_ERR_UNSUPPORTED;
+  if (head_dim != 128 || batch > 65535 || tokens > kMaxPagedKeys || !page_sizes_ok(page_size, kv_head_num, cache_dt)) return LLMHIP_ERR_UNSUPPORTED;
   if ((long long)pages_per_seq * page_size > kMaxPagedKeys) return LLMHIP_ERR_UNSUPPORTED;
   if (page_stride % 16 != 0 || page_stride < (int64_t)llmhip_paged_page_bytes(page_size, kv_head_num, head_dim, cache_dt))
     return LLMHIP_ERR_INVALID_ARG;

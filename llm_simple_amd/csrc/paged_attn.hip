@@ -7,17 +7,24 @@
 // a kv head are read for all g heads at once.  Two kinds of workgroups, of four waves each:
 //
 //  * few rows: a sequence with at most 16 rows.  A stream of K and V through the chip: the rows are the 16 columns of mfma 16x16x32, a wave
-//    takes every fourth piece of 32 keys and keeps its own running maximum, sum and O; the four are merged at the end.  K is loaded as
-//    the operand has it, V goes through LDS of the wave's own and is read transposed.
+//    takes every fourth piece of 32 keys and keeps its own running maximum, sum and O; the four are merged at the end.  V goes through LDS
+//    of the wave's own and is read transposed.
 //  * tiles: 128 rows, 32 to a wave (wave_attn.hpp), over tiles of 64 keys in LDS, two of them, so that a tile is on its way while
 //    the one before it is worked on.
 //
-// 8-bit rows become rows of the storage type on their way into LDS: each is widened once for all rows that use it, by a conversion
-// that takes the row's power of two along, and everything after is the same code.
+// 8-bit rows become rows of the storage type before the matrix instructions: each is widened once by a workgroup, for all rows that use
+// it, by a conversion that takes the row's power of two along, and everything after is the same code.
 //
 // What a workgroup is for is found on the device (lengths may change between replays of a graph), see find_work: a wave looks at 64 sequences
-// at a time.  Where the keys that a tile's rows see are dealt to several workgroups, each leaves an fp32 partial, and a second launch folds
-// them.  A unit of keys is 128 (few rows) or 64.
+// at a time.  Where the keys that a tile's rows see are dealt to several workgroups, each leaves an fp32 partial.  Few rows' are folded by
+// the workgroup that finds all of them stored, tiles' by a second launch, which has the whole chip for them.  A unit of keys is 128 (few rows)
+// or 64.
+//
+// Few rows are bound by the memory system: 16 sequences of 32768 keys of 8 kv heads, 8 bits, 1.08 GB in 170 us, 6.4 TB/s (16 bits 2.15 GB, 326 us,
+// 6.6); a short cache by its chain of memory round trips (starts and lengths, page table, K and V; 384 keys of 2 kv heads 6.7 us, of which an
+// empty launch is 1.6).  Tiles are bound, as the prefill kernels are, by matrix and vector instructions that share a SIMD and the chip's power:
+// a step of two workgroups to a CU takes 2.0-2.2 us, 1.0 PFLOP/s; 4 us of a workgroup's time are its start.  (us: a prompt of 4096 tokens of 28 + 4 heads
+// 132, 0.91 PFLOP/s, in 8 bits 151; 200 past 16001 65; 8192 with a window of 1024 152.)
 //
 // Keys that a row must not see: their scores become -inf, so their K does not matter, but a weight of 0 times a V that is not finite
 // would be NaN.  Rows behind the last key, and pages that are not there, are zeros (the loads' descriptors end before them).  V of keys
@@ -34,7 +41,7 @@
 namespace llmhip {
 
 constexpr int kFewCols = 16;     // rows of a few-rows workgroup
-constexpr int kFlagBytes = 16;
+constexpr int kFlagBytes = 16;   // place of a flag (few_rows_of)
 constexpr int kFewUnit = 128;    // keys of a unit, 32 to a wave
 constexpr int kTileRows = 128;   // rows of a tile
 constexpr int kTileUnit = 64;    // keys of a unit
@@ -45,11 +52,11 @@ constexpr int kFewLds = 8 * kWaveStage, kTilesLds = 4 * kUnitBytes;
 // One kind of work of a launch
 struct PagedKind {
   float *o, *ml;     // partials [slot][kv head][row][128], and [2]: maximum (times scale and log2 e), sum
-  char *flags;       // [slot][kv head], see few_rows
+  char *flags;       // [slot][kv head], see few_rows_of
   int slots;         // room for so many; 0: nothing is split
+  int tiles;         // so many at most, or the grid is too small for them
   int least;         // units that a part has at least
   int parts;         // workgroups of a kv head that run at a time
-  int rounds;        // of these, where parts cannot be made to fit one
 };
 struct PagedAttn {
   PagedBatch batch;
@@ -88,9 +95,6 @@ __device__ __forceinline__ void take_early(PagedAttn &p, addresses_t a, u32x4_t 
   p.batch.keys_max = c[0];
   p.g = c[1];
 }
-
-__device__ __forceinline__ float bits_to_float(int x) { return __builtin_bit_cast(float, x); }
-__device__ __forceinline__ int float_to_bits(float x) { return __builtin_bit_cast(int, x); }
 
 // The keys that rows at positions p0 .. p1 see, in units of UNIT keys: the first `sink_units` of them are keys 0 .. sink_end, the rest
 // begin at key `first`, a multiple of 16, and end at `end`.
@@ -152,10 +156,14 @@ template <bool FEW> struct PagedSeqs {
 };
 
 // Dealing keys to workgroups.  A sequence's tiles are split into as many parts as it has chunks of units; the chunk is the least for which
-// all parts of all tiles (each counted like its sequence's last) run at a time.  Where there are too many tiles for that, the chunk is that of
-// several rounds.  That is at most a part to a tile more than run in those rounds, and a sequence in parts has at least half a chunk to a
+// all parts of all tiles (each counted like its sequence's last) run at a time, or an equal share of all units where there are too many
+// tiles for that.  That is at most a part to a tile more than run at a time, and a sequence in parts has at least half a chunk to a
 // part: at most twice as many partials.  Whoever needs it works it out by itself, with the same instructions, so all agree; a
 // sequence whose partials find no room is not split.
+//
+// Few rows: a workgroup to a CU, in parts of 3 units or more (us, one / two to a CU: 5 x 2999 keys of 8 kv heads in 8 bits 15.6 / 17.2, 48 ragged sequences
+// with a window of 4096 61 / 76; parts of 2: 384 keys of 2 kv heads 8.6 -> 9.4, 5 x 2999 16.8 -> 16.4).  Tiles: two to a CU, 6 units or more (4:
+// 16 prompts of 300 36.6 -> 43; 12: 64 past 4000 of 40 + 8 heads in 8 bits 26.2 -> 32.8; three to a CU beside few rows: 101 -> 116).
 //
 // FOLD: the tile of number w among those that are split.  Else: the part of number w of all; a sequence's last tiles first.
 __device__ __forceinline__ int parts_of(int units, float chunk) {
@@ -164,8 +172,8 @@ __device__ __forceinline__ int parts_of(int units, float chunk) {
 template <typename X> __device__ __forceinline__ X wave_sum(X x) {
   return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_prefix(x)), 63));
 }
-// One sequence by itself: the same in scalar registers, a third of the instructions (which is what workgroups of few tiles
-// wait for: chunk of 200 past 16001, FIGURES).
+// One sequence by itself: the same in scalar registers, a third of the instructions (us, 384 keys of 2 kv heads 7.2 -> 6.8, a prompt of 8192 with a
+// window 155 -> 152; a prompt of 1000 of 40 + 8 heads, whose tiles are half of what runs at a time and are not split, 48 -> 34).
 template <bool FEW, bool FOLD> __device__ __forceinline__ bool find_alone(const PagedAttn &p, int w, PagedTile &t) {
   const PagedKind &kind = FEW ? p.few : p.tiles;
   const int start = p.batch.q_starts[0], end = p.batch.q_starts[1], len = p.batch.kv_lens[0];
@@ -187,9 +195,9 @@ template <bool FEW, bool FOLD> __device__ __forceinline__ bool find_alone(const 
   t.rows = min(rows - t.row0, FEW ? kFewCols : kTileRows);
   return true;
 }
-// Where sequences' lengths leave the greatest chunk well above an equal share, or more parts than run at a time, few-rows workgroups take runs of the units of all sequences
-// one after the other, equal to a unit; a run may end one sequence and begin another, and then costs the start of another.  (us, parts /
-// runs: 48 sequences of up to 16384 keys of 4 kv heads, 48 units to a run, 16 bits 167 / 145, 8 bits 107 / 85; 24 of up to 8192 of 8, 24 units, 76.7 /
+// Where sequences' lengths leave the greatest chunk well above an equal share, or more parts than run at a time, few-rows workgroups
+// take runs of the units of all sequences one after the other, equal to a unit; a run may end one sequence and begin another, and then
+// costs the start of another.  (us, parts / runs: 48 sequences of up to 16384 keys of 4 kv heads, 48 units to a run, 16 bits 167 / 145, 8 bits 107 / 85; 24 of up to 8192 of 8, 24 units, 76.7 /
 // 72.2 and 52.4 / 51.4; with a window of 4096, 20 units, 61.2 / 67.0; 64 of up to 2048 of 2, 4 units, 19.9 / 23.2.)  A kernel of its own, for
 // bounds that allow runs: the loop over sequences costs a call of 7 us 0.6.
 constexpr int kRunUnits = 24;
@@ -232,17 +240,21 @@ __device__ __forceinline__ bool find_work(const PagedAttn &p, int w, int lane, P
   const PagedKind &kind = FEW ? p.few : p.tiles;
   PagedSeqs<FEW> s(p, 0, lane);
   float chunk = 0.0f;
+  bool split = false;
   if (kind.slots) {
     float units = 0.0f;
+    int tiles = 0;
     for (int base = 0;;) {
       units += wave_sum((float)s.tiles * (float)s.units);
+      tiles += wave_sum(s.tiles);
       if ((base += 64) >= p.batch.batch) break;
       s = PagedSeqs<FEW>(p, base, lane);
     }
     const float least = (float)kind.least;
-    chunk = fmaxf(units * __builtin_amdgcn_rcpf((float)(kind.parts * kind.rounds)), least);
+    chunk = fmaxf(units * __builtin_amdgcn_rcpf((float)kind.parts), least);
+    // (More tiles: sequences overlap, which is not allowed.  A part that no workgroup takes would leave the others' flags up.)
+    split = tiles <= kind.tiles;
     if (p.batch.batch <= 64) {
-      const int tiles = wave_sum(s.tiles);
       [[maybe_unused]] bool even = false;
       for (int fit = kind.parts, tries = 0; tries < 6 && 2 * fit > kind.parts && tiles <= kind.parts; ++tries) {
         const float tried = fmaxf(units * __builtin_amdgcn_rcpf((float)fit), least);
@@ -270,7 +282,7 @@ __device__ __forceinline__ bool find_work(const PagedAttn &p, int w, int lane, P
   int slot = 0;
   for (int base = 0; base < p.batch.batch; base += 64) {
     if (base > 0) s = PagedSeqs<FEW>(p, base, lane);
-    int splits = kind.slots ? parts_of(s.units, chunk) : 1;
+    int splits = split ? parts_of(s.units, chunk) : 1;
     const int partials = splits > 1 ? s.tiles * splits : 0;
     const int slots_upto = slot + wave_prefix(partials);
     if (slots_upto > kind.slots) splits = 1;
@@ -364,11 +376,11 @@ __device__ __forceinline__ bool sees(const PagedAttn &p, int pos, int key) {
   return key <= pos && (p.window <= 0 || key > pos - p.window || key < p.sinks);
 }
 
-// One row by G lanes, from the keys that it sees alone; see the header.  dims G * i .. of lane i's: 128 / G of them from 128 / G * i on.
-// M is in units of score times log2 e.
+// One row by G lanes, from the keys that it sees alone; see the header.  Lane i has 128 / G dims from 128 / G * i on.  M is in units of
+// score times log2 e.
 template <typename T, bool EIGHT, int G, int UNIT>
-__device__ __forceinline__ void exact_row(const PagedAttn &p, int b, int kvh, const char *q_row, int pos, PagedKeys keys, int u0, int u1,
-                                                    float &M, float &L, float (&o)[kHeadDim / G]) {
+__device__ __forceinline__ void exact_row(const PagedAttn &p, int b, int kvh, const char *q_row, int pos, PagedKeys keys, int u0, int u1, float &M,
+                                          float &L, float (&o)[kHeadDim / G]) {
   constexpr int D = kHeadDim / G, W = cached_row_bytes(EIGHT);
   const int lane = threadIdx.x & (G - 1);
   const size_t exponents = (size_t)p.Hkv * p.batch.page_size.d * kHeadDim;
@@ -439,8 +451,11 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows_of(co
   using E = Elem<T>;
   constexpr int kLoads = EIGHT ? 4 : 8;  // of 1 KiB, for 32 rows
   constexpr int W = cached_row_bytes(EIGHT);
+  // 16 bits: K through LDS like V, whole 1 KiB pieces to a load, one step on its way (us, loaded as the operand has it, 64 bytes of 16
+  // rows / this: 48 ragged sequences with a window 72 / 61, without 185 / 167; 16 x 32768 keys 315 / 327).  8 bits: as the operand has it, and two steps on
+  // their way, as many bytes (16 x 32768, through LDS 175 / 169, one step 190; 48 ragged 120 / 107).
   constexpr bool kStaged = !EIGHT;
-  constexpr int kAhead = EIGHT ? 2 : 1;  // steps on their way
+  constexpr int kAhead = EIGHT ? 2 : 1;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, cg = lane >> 4;
   const int p0 = t.len - t.m, p1 = t.len - 1;
   const PagedKeys keys = keys_seen<kFewUnit>(p, p0, p1, t.len);
@@ -1074,7 +1089,7 @@ template <typename T> __global__ __launch_bounds__(256) void paged_combine_kerne
 struct PagedPlan {
   struct Kind {
     long long tiles, items, slots, rows;  // at most; rows of a partial
-    int least, parts, rounds;
+    int least, parts;
     bool flags;
     size_t bytes(int Hkv) const { return (size_t)slots * Hkv * (rows * (kHeadDim + 2) * sizeof(float) + (flags ? kFlagBytes : 0)); }
     long long folds() const { return slots / 2 < tiles ? slots / 2 : tiles; }  // tiles that are split, at most
@@ -1089,23 +1104,22 @@ static PagedPlan plan_paged(int tokens, int batch, int max_q_len, int max_kv_len
   // (all sequences have max_q_len tokens, or the tokens do not add up: no few-rows ones)
   if (!tiles || (g <= kFewCols && (long long)batch * max_q_len != tokens)) pl.few.tiles = sequences;
   if (tiles) pl.by_tiles.tiles = (long long)tokens * g / kTileRows + sequences;
-  auto deal = [&](PagedPlan::Kind &kind, int rows, int unit, long long span, long long workgroups, int rounds, int least) {
+  auto deal = [&](PagedPlan::Kind &kind, int rows, int unit, long long span, long long workgroups, int least) {
     kind.rows = rows;
     kind.flags = rows == kFewCols;
     kind.least = least;
     kind.parts = Hkv <= workgroups ? (int)(workgroups / Hkv) : 1;
-    kind.rounds = rounds;
     const long long windowed = (long long)window + span + sinks + 2 * kPageGroup, seen = window > 0 && windowed < max_kv_len ? windowed : max_kv_len;
-    const long long units = (seen + unit - 1) / unit, all = (long long)kind.parts * rounds + 1 + kind.parts * rounds / 64;
+    const long long units = (seen + unit - 1) / unit, all = (long long)kind.parts + 1 + kind.parts / 64;
     kind.slots = kind.tiles > 0 && units > least && Hkv <= workgroups ? 2 * all : 0;
     const long long most = kind.tiles * (units / least + 1);
     if (kind.slots > most) kind.slots = most;
     kind.items = kind.tiles + (kind.slots ? all : 0);
     return units;
   };
-  const long long units = deal(pl.few, kFewCols, kFewUnit, kFewCols, cus, 1, 3);
+  const long long units = deal(pl.few, kFewCols, kFewUnit, kFewCols, cus, 3);
   pl.runs = batch > 1 && batch <= 64 && pl.few.slots > 0 && pl.few.tiles * units >= (long long)kRunUnits * pl.few.parts;
-  deal(pl.by_tiles, kTileRows, kTileUnit, kTileRows / g + 1, 2 * cus, 1, 6);
+  deal(pl.by_tiles, kTileRows, kTileUnit, kTileRows / g + 1, 2 * cus, 6);
   return pl;
 }
 
@@ -1134,7 +1148,7 @@ hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, cons
   float *ws = static_cast<float *>(workspace);
   auto kind_of = [&](const PagedPlan::Kind &k) {
     float *const ml = ws + (size_t)k.slots * Hkv * k.rows * kHeadDim;
-    const PagedKind kind = {ws, ml, reinterpret_cast<char *>(ml + (size_t)k.slots * Hkv * k.rows * 2), (int)k.slots, k.least, k.parts, k.rounds};
+    const PagedKind kind = {ws, ml, reinterpret_cast<char *>(ml + (size_t)k.slots * Hkv * k.rows * 2), (int)k.slots, (int)k.tiles, k.least, k.parts};
     if (k.slots) ws += k.bytes(Hkv) / sizeof(float);
     return kind;
   };
@@ -1142,7 +1156,7 @@ hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, cons
   p.tiles = kind_of(pl.by_tiles);
   const long long few_blocks = pl.few.items * Hkv, tile_blocks = pl.by_tiles.items * Hkv;
   const long long folds = pl.by_tiles.folds() * Hkv * (kTileRows / 8);
-  if (few_blocks + tile_blocks > 0x7fffffffLL || folds > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (pl.few.tiles + pl.by_tiles.tiles > 0x7fffffffLL || few_blocks + tile_blocks > 0x7fffffffLL || folds > 0x7fffffffLL) return hipErrorInvalidValue;
   p.number = pl.few.slots ? launch_number() : 0;
   p.few_blocks = (int)few_blocks;
   auto kernel_of = [&](auto mode) {

@@ -26,7 +26,7 @@ COMMON = [("tokens", 0, -1), ("batch", 0, -1), ("pages_per_seq", 0, -1), ("num_p
           ("page_stride", -16 * 2 * 256, -1), ("head_dim", 64, -2), ("cache_dt", 4, -1), ("cache_dt", 0, -1), ("dt", 6, -1), ("dt", 16, -1),
           ("pages_per_seq", (1 << 26) + 1, -2), ("q_starts", 2, -1), ("kv_lens", 1, -1), ("page_table", 2, -1), ("k_pages", 8, -1),
           ("v_pages", 4, -1), ("k_pages", None, -1), ("v_pages", None, -1), ("page_table", None, -1), ("q_starts", None, -1),
-          ("kv_lens", None, -1)]
+          ("kv_lens", None, -1), ("batch", 65536, -2), ("tokens", (1 << 30) + 1, -2)]
 OWN = [("llmhip_paged_rope_kv_append", *x) for x in [
            ("table_rows", 0, -1), ("n_heads", 0, -1), ("n_kv_heads", 0, -1), ("n_kv_heads", 65536, -2), ("n_heads", 65536, -2),
            ("out_q", None, -1), ("in_q", 2, -1), ("in_k", None, -1), ("in_v", 8, -1), ("freq_cis", 4, -1)]] + \
