@@ -69,6 +69,7 @@ struct PagedAttn {
   int max_q_len;
   int few_rows;    // sequences of up to so many rows are few-rows ones; 0: none is
   int few_blocks;  // workgroups of few rows, the first ones in a launch of both
+  int fold_shift;  // 2^this times 8 rows to a workgroup that folds
   uint64_t number;  // of the launch
 };
 // What the first loads of a workgroup need, in its registers when it starts (common.hpp).
@@ -1041,14 +1042,7 @@ template <typename T, bool EIGHT, PagedMode MODE> __global__ __launch_bounds__(2
     tile_rows<T, EIGHT>(p, unit - (MODE == kBoth ? p.few_blocks : 0), lds);
 }
 
-// Partials of a tile of a kv head, 8 rows to a workgroup, 32 lanes of 4 dims to a row; 8 partials are on their way at a time.
-template <typename T> __global__ __launch_bounds__(256) void paged_combine_kernel(addresses_t a, u32x4_t b, u32x2_t c_, PagedAttn p) {
-  take_early(p, a, b, c_);
-  const int tid = threadIdx.x, lane = tid & 63, d4 = (tid & 31) * 4;
-  const int unit = blockIdx.x / (kTileRows / 8), c = blockIdx.x % (kTileRows / 8) * 8 + (tid >> 5);
-  const int item = (int)fast_div(unit, p.Hkv_div), kvh = unit - item * p.Hkv;
-  PagedTile t;
-  if (!find_work<false, true>(p, item, lane, t) || c >= t.rows) return;
+template <typename T> __device__ __forceinline__ void fold_row(const PagedAttn &p, const PagedTile &t, int kvh, int c, int d4) {
   const size_t row = ((size_t)t.slot * p.Hkv + kvh) * kTileRows + c, step = (size_t)p.Hkv * kTileRows;
   const float *po = p.tiles.o + row * kHeadDim + d4, *pml = p.tiles.ml + row * 2;
   float M = -INFINITY, L = 0.0f;
@@ -1083,6 +1077,19 @@ template <typename T> __global__ __launch_bounds__(256) void paged_combine_kerne
   const int tok = (int)fast_div(t.row0 + c, p.g_div);
   const u32x2_t w = {Elem<T>::pack2(acc[0] * inv, acc[1] * inv), Elem<T>::pack2(acc[2] * inv, acc[3] * inv)};
   *reinterpret_cast<u32x2_t *>(p.out + ((size_t)(t.start + tok) * p.H + kvh * p.g + t.row0 + c - tok * p.g) * kRowBytes + d4 * 2) = w;
+}
+// Partials of a tile of a kv head, 8 rows to a workgroup, or 16 or 32 one after the other, 32 lanes of 4 dims to a row; 8 partials are on
+// their way at a time.  The more tiles the host counts with, the fewer are split, and a workgroup that finds nothing to fold costs its
+// start (us, 8 rows / 16 / 32, tiles of a kv head by the parts that run at a time: a prompt of 4096, 1.8, 135.5 / 133.3 / 133.2; six of up to 1019 of 32 kv heads, 2.7,
+// 71.5 / 70.2 / 67.4; 6 x 700 past 2000, 1.8, 100.8 / 99.1 / 100.6; 4 x 400 past 3000, 0.7, 104.9 / 102.5 / 102; 200 past 16001, 0.1, 64.9 / 67.0 / 69.2).
+template <typename T> __global__ __launch_bounds__(256) void paged_combine_kernel(addresses_t a, u32x4_t b, u32x2_t c_, PagedAttn p) {
+  take_early(p, a, b, c_);
+  const int tid = threadIdx.x, lane = tid & 63, d4 = (tid & 31) * 4;
+  const int unit = (int)(blockIdx.x << p.fold_shift) / (kTileRows / 8), item = (int)fast_div(unit, p.Hkv_div), kvh = unit - item * p.Hkv;
+  PagedTile t;
+  if (!find_work<false, true>(p, item, lane, t)) return;
+  const int c0 = (int)(blockIdx.x << p.fold_shift) % (kTileRows / 8) * 8, c1 = min(c0 + (8 << p.fold_shift), t.rows);
+  for (int c = c0 + (tid >> 5); c < c1; c += 8) fold_row<T>(p, t, kvh, c, d4);
 }
 
 // How a launch is shaped, from what the host knows: bounds, not lengths.
@@ -1155,7 +1162,8 @@ hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, cons
   p.few = kind_of(pl.few);
   p.tiles = kind_of(pl.by_tiles);
   const long long few_blocks = pl.few.items * Hkv, tile_blocks = pl.by_tiles.items * Hkv;
-  const long long folds = pl.by_tiles.folds() * Hkv * (kTileRows / 8);
+  p.fold_shift = pl.by_tiles.tiles > 2 * pl.by_tiles.parts ? 2 : 2 * pl.by_tiles.tiles > pl.by_tiles.parts ? 1 : 0;
+  const long long folds = pl.by_tiles.folds() * Hkv * (kTileRows / 8 >> p.fold_shift);
   if (pl.few.tiles + pl.by_tiles.tiles > 0x7fffffffLL || few_blocks + tile_blocks > 0x7fffffffLL || folds > 0x7fffffffLL) return hipErrorInvalidValue;
   p.number = pl.few.slots ? launch_number() : 0;
   p.few_blocks = (int)few_blocks;
