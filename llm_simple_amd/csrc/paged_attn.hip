@@ -894,9 +894,6 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
     issue_k(nxt.g, 1);
     issue_exponents(nxt.g, cur.g);
     widen_k(1);
-    // (the compiler knows nothing of the waits below, and would wait for Q, and with it for the tiles on their way, in the loop)
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) asm volatile("" : "+v"(w.qf[kk]));
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (w_iters > 0) w.qk(lds, 0, sa);
     // K(2) goes where tile 0 was just read: no wave may issue it before all have
@@ -941,6 +938,10 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
     after = next_of(it + 3);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
+  // (The compiler knows nothing of the waits above, and would wait for Q, and with it for the tiles on their way, in the loop.  Here, where
+  // there are no tiles too: it would do so on their account.)
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) asm volatile("" : "+v"(w.qf[kk]));
   for (int it = 0; it < iters; it += 2) {
     step(it, std::integral_constant<int, 0>(), sa, sb);
     if (it + 1 < iters) step(it + 1, std::integral_constant<int, 1>(), sb, sa);
