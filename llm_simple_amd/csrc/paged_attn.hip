@@ -490,8 +490,9 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows_of(co
     u32x4_t k[kLoads], v[kLoads];
     uint8_t k_exps[2], v_exps[2];  // 8 bits: bytes of rows col (K) and lane % 16 (V) of either group
   };
+  // (Steps past the last find no groups: loads of nothing.  No branch round the loads, and K's before V's, so that the compiler can count
+  // them, and waits for a step's alone.)
   auto fetch = [&](Step &s, int it) {
-    if (it >= iters) return;
     if ((it & 31) == 0 && it > 0) {
       places = group_places<EIGHT>(p, later);
       later = look(it + 32);
@@ -504,6 +505,7 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows_of(co
       for (int i = 0; i < kLoads / 2; ++i) s.k[half * (kLoads / 2) + i] = stream_load(r, kStaged ? i * 1024 + lane * 16 : col * W + cg * 16 + i * 64);
       if constexpr (EIGHT) s.k_exps[half] = __builtin_amdgcn_raw_buffer_load_b8(byte_buffer(group_exponents(p, p.k, s.g[half]), s.g[half].have()), col, 0, 0);
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const __amdgpu_buffer_rsrc_t r = group_buffer<EIGHT>(p.v, s.g[half]);
@@ -608,11 +610,16 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows_of(co
     later = look(32);
     Step a = {}, b = {};
     fetch(a, 0);
-    if (kAhead > 1) fetch(b, 1);
-    for (int it = 0; it < iters; it += kAhead) {
-      step(a, it);
-      if (kAhead > 1 && it + 1 < iters) step(b, it + 1);
+    if (kAhead > 1) {
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(b, 1);
     }
+    int it = 0;
+    for (; it + kAhead <= iters; it += kAhead) {
+      step(a, it);
+      if (kAhead > 1) step(b, it + 1);
+    }
+    if (kAhead > 1 && it < iters) step(a, it);
   }
 
   // ---- merge the waves: [wave][col][128], the pieces of a row XORed with the column ----
@@ -878,6 +885,10 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
   const int w_keys = w_p1 + 1;
   const int w_units = w_keys > keys.first ? keys.sink_units + (w_keys - keys.first + kTileUnit - 1) / kTileUnit : (max(w_keys, 0) + kTileUnit - 1) / kTileUnit;
   const int w_iters = max(0, min(iters, w_units - part.u0));
+  // tiles from clear0 to clear1 are seen whole by all of this wave's rows, as far as they are there
+  const int clear0 = (p.window > 0 ? keys.sink_units + max(((w_p1 - p.window - keys.first) >> 6) + 1, 0) : 0) - part.u0;
+  const int clear1 = keys.sink_units + max((min(w_p0 + 1, keys.end) - keys.first) >> 6, 0) - part.u0;
+  static_assert(kTileUnit == 64);
   f32x16_t sa[2], sb[2];
   Next cur = {}, nxt = {}, after = {};  // of tiles j, j + 1 and j + 2
   float scale = kScaleLog2e;
@@ -905,8 +916,8 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
     issue_v(nxt.g, slot ^ 1);
     issue_exponents(after.g, nxt.g);
     if (it < w_iters) {
-      const int u = part.u0 + it, base = keys.base(u, kTileUnit), limit = keys.limit(u);
-      if (base + kTileUnit > min(w_p0 + 1, limit) || cur.there != 15 || (p.window > 0 && base <= w_p1 - p.window && base + kTileUnit > p.sinks)) {
+      if (it < clear0 || it >= clear1 || cur.there != 15) {
+        const int u = part.u0 + it, base = keys.base(u, kTileUnit), limit = keys.limit(u);
         const int from = base + 4 * w.hh;
         // a lane's keys are 8 * (i / 4) + i % 4 of 32 from its first one on
         auto hide = [&](auto hidden) {
