@@ -21,10 +21,10 @@
 // or 64.
 //
 // Few rows are bound by the memory system: 16 sequences of 32768 keys of 8 kv heads, 8 bits, 1.08 GB in 170 us, 6.4 TB/s (16 bits 2.15 GB, 326 us,
-// 6.6); a short cache by its chain of memory round trips (starts and lengths, page table, K and V; 384 keys of 2 kv heads 6.7 us, of which an
+// 6.6); a short cache by its chain of memory round trips (starts and lengths, page table, K and V; 384 keys of 2 kv heads 6.5 us, of which an
 // empty launch is 1.6).  Tiles are bound, as the prefill kernels are, by matrix and vector instructions that share a SIMD and the chip's power:
 // a step of two workgroups to a CU takes 2.0-2.2 us, 1.0 PFLOP/s; 4 us of a workgroup's time are its start.  (us: a prompt of 4096 tokens of 28 + 4 heads
-// 132, 0.91 PFLOP/s, in 8 bits 151; 200 past 16001 65; 8192 with a window of 1024 152.)
+// 133, 0.90 PFLOP/s, in 8 bits 149; 200 past 16001 66; 8192 with a window of 1024 150.)
 //
 // Keys that a row must not see: their scores become -inf, so their K does not matter, but a weight of 0 times a V that is not finite
 // would be NaN.  Rows behind the last key, and pages that are not there, are zeros (the loads' descriptors end before them).  V of keys
