@@ -157,3 +157,15 @@ def test_a_batch_of_overlapping_sequences_leaves_nothing_behind():
         torch.cuda.synchronize()
         if turn % 2:
             s.check(out, expected=expected)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("tokens,unit,each", [(1, 128, 32), (20, 64, 16)])
+@pytest.mark.parametrize("more", [(0, 0), (0, 1), (1, -1), (1, 7), (2, 0)])
+def test_one_workgroup_past_what_it_looks_up_at_a_time(tokens, unit, each, more, eight):
+    """A bound of a few keys: nothing is split, and a workgroup takes all of a sequence, about as many units as it looks up at once, or twice."""
+    s = Setup(40, [(unit * (each + each * (more[0] > 0) + more[0] - 1) + more[1], tokens), (unit * each - 3, tokens)], 1, 2, BF16, eight, 32).to_gpu()
+    assert s.workspace(max_kv=unit)[1] == 0
+    out = s.out()
+    s.attend(out, max_kv=unit)
+    s.check(out)
