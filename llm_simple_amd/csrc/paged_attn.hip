@@ -4,13 +4,13 @@
 //   out[t][h] = sum_c softmax_c(q[t][h] . K[c][h / g] / sqrt(128)) V[c][h / g],   c <= p, and c > p - window or c < sinks
 //
 // with p the position of token t (paged.hpp).  Query rows of a kv head are (token, head of its g) pairs, token-major, so that K and V of
-// a kv head are read for all g heads at once.  Two kinds of workgroups, of four waves each:
+// a kv head are read for all g heads at once.  Two kinds of workgroups, of four waves:
 //
 //  * few rows: a sequence with at most 16 rows.  A stream of K and V through the chip: the rows are the 16 columns of mfma 16x16x32, a wave
 //    takes every fourth piece of 32 keys and keeps its own running maximum, sum and O; the four are merged at the end.  V goes through LDS
 //    of the wave's own and is read transposed.
 //  * tiles: 128 rows, 32 to a wave (wave_attn.hpp), over tiles of 64 keys in LDS, two of them, so that a tile is on its way while
-//    the one before it is worked on.
+//    the one before it is worked on.  Wide ones have 256 rows and eight waves (plan_paged).
 //
 // 8-bit rows become rows of the storage type before the matrix instructions: each is widened once by a workgroup, for all rows that use
 // it, by a conversion that takes the row's power of two along, and everything after is the same code.
@@ -23,8 +23,8 @@
 // Few rows are bound by the memory system: 16 sequences of 32768 keys of 8 kv heads, 8 bits, 1.08 GB in 170 us, 6.4 TB/s (16 bits 2.15 GB, 326 us,
 // 6.6); a short cache by its chain of memory round trips (starts and lengths, page table, K and V; 384 keys of 2 kv heads 6.5 us, of which an
 // empty launch is 1.6).  Tiles are bound, as the prefill kernels are, by matrix and vector instructions that share a SIMD and the chip's power:
-// a step of two workgroups to a CU takes 2.0-2.2 us, 1.0 PFLOP/s; 4 us of a workgroup's time are its start.  (us: a prompt of 4096 tokens of 28 + 4 heads
-// 133, 0.90 PFLOP/s, in 8 bits 149; 200 past 16001 66; 8192 with a window of 1024 150.)
+// a step of two workgroups to a CU takes 2.0-2.2 us, 1.0 PFLOP/s; 4 us of a workgroup's time are its start.  (us: a prompt of 4096 tokens of 28 + 4
+// heads 134, 0.90 PFLOP/s, in 8 bits 131; 200 past 16001 63.5; 8192 with a window of 1024 150.)
 //
 // Keys that a row must not see: their scores become -inf, so their K does not matter, but a weight of 0 times a V that is not finite
 // would be NaN.  Rows behind the last key, and pages that are not there, are zeros (the loads' descriptors end before them).  V of keys
@@ -43,7 +43,7 @@ namespace llmhip {
 constexpr int kFewCols = 16;     // rows of a few-rows workgroup
 constexpr int kFlagBytes = 16;   // place of a flag (few_rows_of)
 constexpr int kFewUnit = 128;    // keys of a unit, 32 to a wave
-constexpr int kTileRows = 128;   // rows of a tile
+constexpr int kTileRows = 128;   // rows of a tile (wide: twice as many)
 constexpr int kTileUnit = 64;    // keys of a unit
 constexpr int kUnitBytes = kTileUnit * kRowBytes;
 constexpr int kWaveStage = 32 * kRowBytes;  // staging of a few-rows wave, for K and for V
@@ -68,6 +68,7 @@ struct PagedAttn {
   int window, sinks;  // window 0: none
   int max_q_len;
   int few_rows;    // sequences of up to so many rows are few-rows ones; 0: none is
+  int tile_shift;  // a tile has 2^this rows
   int few_blocks;  // workgroups of few rows, the first ones in a launch of both
   int fold_shift;  // 2^this times 8 rows to a workgroup that folds
   uint64_t number;  // of the launch
@@ -150,8 +151,8 @@ template <bool FEW> struct PagedSeqs {
     const bool valid = base + lane < p.batch.batch && sequence_ok(p.batch, start, end, len) && end - start <= p.max_q_len;
     m = valid ? end - start : 0;
     const int rows = m * p.g;
-    tiles = FEW ? (m > 0 && rows <= p.few_rows ? 1 : 0) : rows <= p.few_rows ? 0 : (rows + kTileRows - 1) / kTileRows;
-    const int first = FEW ? 0 : (int)fast_div(max(tiles - 1, 0) * kTileRows, p.g_div);
+    tiles = FEW ? (m > 0 && rows <= p.few_rows ? 1 : 0) : rows <= p.few_rows ? 0 : (rows + (1 << p.tile_shift) - 1) >> p.tile_shift;
+    const int first = FEW ? 0 : (int)fast_div(max(tiles - 1, 0) << p.tile_shift, p.g_div);
     units = tiles ? keys_seen<FEW ? kFewUnit : kTileUnit>(p, len - m + first, len - 1, len).units : 0;
   }
 };
@@ -162,9 +163,9 @@ template <bool FEW> struct PagedSeqs {
 // part: at most twice as many partials.  Whoever needs it works it out by itself, with the same instructions, so all agree; a
 // sequence whose partials find no room is not split.
 //
-// Few rows: a workgroup to a CU, in parts of 3 units or more (us, one / two to a CU: 5 x 2999 keys of 8 kv heads in 8 bits 15.6 / 17.2, 48 ragged sequences
-// with a window of 4096 61 / 76; parts of 2: 384 keys of 2 kv heads 8.6 -> 9.4, 5 x 2999 16.8 -> 16.4).  Tiles: two to a CU, 6 units or more (4:
-// 16 prompts of 300 36.6 -> 43; 12: 64 past 4000 of 40 + 8 heads in 8 bits 26.2 -> 32.8; three to a CU beside few rows: 101 -> 116).
+// Few rows: a workgroup to a CU, in parts of 3 units or more (us, one / two to a CU: 5 x 2999 keys of 8 kv heads in 8 bits 15.6 / 17.2, 48 ragged
+// sequences with a window of 4096 61 / 76; parts of 2: 384 keys of 2 kv heads 8.6 -> 9.4, 5 x 2999 16.8 -> 16.4).  Tiles: two to a CU, 6 units or
+// more (4: 16 prompts of 300 36.6 -> 43; 12: 64 past 4000 of 40 + 8 heads in 8 bits 26.2 -> 32.8; three to a CU beside few rows: 101 -> 116).
 //
 // FOLD: the tile of number w among those that are split.  Else: the part of number w of all; a sequence's last tiles first.
 __device__ __forceinline__ int parts_of(int units, float chunk) {
@@ -181,7 +182,7 @@ template <bool FEW, bool FOLD> __device__ __forceinline__ bool find_alone(const 
   if (!sequence_ok(p.batch, start, end, len) || end <= start || end - start > p.max_q_len) return false;
   const int m = end - start, rows = m * p.g;
   if (FEW != (rows <= p.few_rows)) return false;
-  const int tiles = FEW ? 1 : (rows + kTileRows - 1) / kTileRows, first = FEW ? 0 : (int)fast_div((tiles - 1) * kTileRows, p.g_div);
+  const int tiles = FEW ? 1 : (rows + (1 << p.tile_shift) - 1) >> p.tile_shift, first = FEW ? 0 : (int)fast_div((tiles - 1) << p.tile_shift, p.g_div);
   int splits = 1;
   if (kind.slots && tiles <= kind.parts / 2) {
     const int units = keys_seen<FEW ? kFewUnit : kTileUnit>(p, len - m + first, len - 1, len).units;
@@ -191,16 +192,16 @@ template <bool FEW, bool FOLD> __device__ __forceinline__ bool find_alone(const 
   if (FOLD && splits == 1) return false;
   const int tile = FOLD || splits == 1 ? w : w / splits;
   if (tile >= tiles) return false;
-  t = PagedTile{0, start, m, len, FEW ? 0 : (tiles - 1 - tile) * kTileRows, 0, FOLD ? 0 : w - tile * splits, splits, tile * splits};
+  t = PagedTile{0, start, m, len, FEW ? 0 : (tiles - 1 - tile) << p.tile_shift, 0, FOLD ? 0 : w - tile * splits, splits, tile * splits};
   if (!FOLD && splits == 1) t.split = 0;
-  t.rows = min(rows - t.row0, FEW ? kFewCols : kTileRows);
+  t.rows = min(rows - t.row0, FEW ? kFewCols : 1 << p.tile_shift);
   return true;
 }
 // Where sequences' lengths leave the greatest chunk well above an equal share, or more parts than run at a time, few-rows workgroups
 // take runs of the units of all sequences one after the other, equal to a unit; a run may end one sequence and begin another, and then
-// costs the start of another.  (us, parts / runs: 48 sequences of up to 16384 keys of 4 kv heads, 48 units to a run, 16 bits 167 / 145, 8 bits 107 / 85; 24 of up to 8192 of 8, 24 units, 76.7 /
-// 72.2 and 52.4 / 51.4; with a window of 4096, 20 units, 61.2 / 67.0; 64 of up to 2048 of 2, 4 units, 19.9 / 23.2.)  A kernel of its own, for
-// bounds that allow runs: the loop over sequences costs a call of 7 us 0.6.
+// costs the start of another.  (us, parts / runs: 48 sequences of up to 16384 keys of 4 kv heads, 48 units to a run, 16 bits 167 / 145, 8 bits 107 /
+// 85; 24 of up to 8192 of 8, 24 units, 76.7 / 72.2 and 52.4 / 51.4; with a window of 4096, 20 units, 61.2 / 67.0; 64 of up to 2048 of 2, 4 units,
+// 19.9 / 23.2.)  A kernel of its own, for bounds that allow runs: the loop over sequences costs a call of 7 us 0.6.
 constexpr int kRunUnits = 24;
 struct FewRuns {
   PagedSeqs<true> s;
@@ -305,8 +306,8 @@ __device__ __forceinline__ bool find_work(const PagedAttn &p, int w, int lane, P
     const int tile = FOLD || t.splits == 1 ? at : at / t.splits;
     t.split = FOLD ? 0 : at - tile * t.splits;
     t.slot = of(slots_upto) - of(partials) + tile * t.splits;
-    t.row0 = FEW ? 0 : (of(s.tiles) - 1 - tile) * kTileRows;
-    t.rows = min(t.m * p.g - t.row0, FEW ? kFewCols : kTileRows);
+    t.row0 = FEW ? 0 : (of(s.tiles) - 1 - tile) << p.tile_shift;
+    t.rows = min(t.m * p.g - t.row0, FEW ? kFewCols : 1 << p.tile_shift);
     return true;
   }
   return false;
@@ -453,8 +454,8 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows_of(co
   constexpr int kLoads = EIGHT ? 4 : 8;  // of 1 KiB, for 32 rows
   constexpr int W = cached_row_bytes(EIGHT);
   // 16 bits: K through LDS like V, whole 1 KiB pieces to a load, one step on its way (us, loaded as the operand has it, 64 bytes of 16
-  // rows / this: 48 ragged sequences with a window 72 / 61, without 185 / 167; 16 x 32768 keys 315 / 327).  8 bits: as the operand has it, and two steps on
-  // their way, as many bytes (16 x 32768, through LDS 175 / 169, one step 190; 48 ragged 120 / 107).
+  // rows / this: 48 ragged sequences with a window 72 / 61, without 185 / 167; 16 x 32768 keys 315 / 327).  8 bits: as the operand has it, and two
+  // steps on their way, as many bytes (16 x 32768, through LDS 175 / 169, one step 190; 48 ragged 120 / 107).
   constexpr bool kStaged = !EIGHT;
   constexpr int kAhead = EIGHT ? 2 : 1;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, cg = lane >> 4;
@@ -761,23 +762,30 @@ template <typename T, bool EIGHT, bool RUNS> __device__ __forceinline__ void few
 }
 // ---- tiles ----
 
-// 16 rows of a group into LDS, four times 1 KiB, lane by lane: the instruction's offset moves both addresses.  Inline: the compiler would
+// N (4 or 2) times 4 rows of a group into LDS, 1 KiB each, lane by lane: the instruction's offset moves both addresses.  Inline: the compiler would
 // order every later LDS read behind the loads; they are waited for where the waves meet (s_waitcnt vmcnt before a barrier).
-__device__ __forceinline__ void load_group(u32x4_t r, int o0, int o1, int o2, int o3, uint32_t lds_at) {
-  asm volatile(
-      "s_mov_b32 m0, %5\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %4, 0 offen lds\n\tbuffer_load_dwordx4 %1, %4, 0 offen offset:1024 lds\n\t"
-      "buffer_load_dwordx4 %2, %4, 0 offen offset:2048 lds\n\tbuffer_load_dwordx4 %3, %4, 0 offen offset:3072 lds"
-      :
-      : "v"(o0), "v"(o1), "v"(o2), "v"(o3), "s"(r), "s"(lds_at)
-      : "m0", "memory");
+template <int N> __device__ __forceinline__ void load_group(u32x4_t r, const int (&o)[N], uint32_t lds_at) {
+  if constexpr (N == 2)
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds\n\tbuffer_load_dwordx4 %1, %2, 0 offen offset:1024 lds"
+                 :
+                 : "v"(o[0]), "v"(o[1]), "s"(r), "s"(lds_at)
+                 : "m0", "memory");
+  else
+    asm volatile(
+        "s_mov_b32 m0, %5\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %4, 0 offen lds\n\tbuffer_load_dwordx4 %1, %4, 0 offen offset:1024 lds\n\t"
+        "buffer_load_dwordx4 %2, %4, 0 offen offset:2048 lds\n\tbuffer_load_dwordx4 %3, %4, 0 offen offset:3072 lds"
+        :
+        : "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]), "s"(r), "s"(lds_at)
+        : "m0", "memory");
 }
 
 // The loop is that of the prefill kernels: K runs one tile ahead of V, so that the matrix instructions of S(j + 1) = K(j + 1) Q^T stand
 // beside the softmax of tile j, and those of P(j) V(j) beside the exponentials.  In a step, K(j + 2) goes where K(j) was and V(j + 1) where
 // V(j - 1) was, both read in the step before.
-template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(const PagedAttn &p, int unit, char *lds) {
+template <typename T, bool EIGHT, int WAVES> __device__ __forceinline__ void tile_rows(const PagedAttn &p, int unit, char *lds) {
   using E = Elem<T>;
   constexpr int kVRegion = 2 * kUnitBytes;
+  constexpr int kPieces = 16 / WAVES, kPieces8 = 8 / WAVES;  // loads of a wave for K or V of a tile, in 16 and in 8 bits
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int item = (int)fast_div(unit, p.Hkv_div), kvh = unit - item * p.Hkv;
   PagedTile t;
@@ -813,15 +821,18 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
   }
   const int my_pos = before + my_tok;
 
-  // Wave i fetches group i of every tile: 16 rows of K and of V.  Lane offsets within 4 rows (16 bits), which undo the swizzle of
-  // the LDS rows.
+  // A wave fetches a group of every tile, 16 rows of K and of V, or with 8 waves half of one.  Lane offsets within 4 rows (16 bits), which
+  // undo the swizzle of the LDS rows.
+  const int group = wave * 4 / WAVES, part_row = wave * 64 / WAVES - 16 * group;
   const int r4 = lane >> 4, c16 = lane & 15;
-  int k_off[4];
+  int k_off[kPieces], v_off[kPieces];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) k_off[i] = r4 * kRowBytes + ((c16 ^ (4 * i + r4)) << 4);
-  const int v_off = r4 * kRowBytes + (((((c16 >> 2) ^ r4) << 2) | (c16 & 3)) << 4);
-  const uint32_t lds_k = __builtin_amdgcn_readfirstlane(lds_address(lds) + wave * kPageGroup * kRowBytes), lds_v = lds_k + kVRegion;
-  u32x4_t kn[2], vn[2];  // 8 bits: what is on its way to slots of K and V
+  for (int i = 0; i < kPieces; ++i) {
+    k_off[i] = (part_row + r4) * kRowBytes + ((c16 ^ (part_row + 4 * i + r4)) << 4);
+    v_off[i] = (part_row + r4) * kRowBytes + (((((c16 >> 2) ^ r4) << 2) | (c16 & 3)) << 4);
+  }
+  const uint32_t lds_k = __builtin_amdgcn_readfirstlane(lds_address(lds) + (16 * group + part_row) * kRowBytes), lds_v = lds_k + kVRegion;
+  u32x4_t kn[kPieces8], vn[kPieces8];  // 8 bits: what is on its way to slots of K and V
   int exps = 0;
 
   GroupPlaces places = {0, 0, 0};
@@ -836,7 +847,7 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
       later = look(it + 16);
     }
     Next n;
-    n.g = group_at(places, (it & 15) * 4 + wave);
+    n.g = group_at(places, (it & 15) * 4 + group);
     n.there = (uint32_t)(__builtin_amdgcn_ballot_w64(places.rest != 0) >> ((it & 15) * 4)) & 15u;
     return n;
   };
@@ -844,18 +855,20 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
     if constexpr (EIGHT) {
       const __amdgpu_buffer_rsrc_t r = group_buffer<true>(p.k, g);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) kn[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, i * 1024 + lane * 16, 0, 0));
+      for (int i = 0; i < kPieces8; ++i)
+        kn[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, part_row * kHeadDim + i * 1024 + lane * 16, 0, 0));
     } else {
-      load_group(group_words(p.k, g), k_off[0], k_off[1], k_off[2], k_off[3], lds_k + slot * kUnitBytes);
+      load_group<kPieces>(group_words(p.k, g), k_off, lds_k + slot * kUnitBytes);
     }
   };
   auto issue_v = [&](const Group &g, int slot) {
     if constexpr (EIGHT) {
       const __amdgpu_buffer_rsrc_t r = group_buffer<true>(p.v, g);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) vn[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, i * 1024 + lane * 16, 0, 0));
+      for (int i = 0; i < kPieces8; ++i)
+        vn[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, part_row * kHeadDim + i * 1024 + lane * 16, 0, 0));
     } else {
-      load_group(group_words(p.v, g), v_off, v_off, v_off, v_off, lds_v + slot * kUnitBytes);
+      load_group<kPieces>(group_words(p.v, g), v_off, lds_v + slot * kUnitBytes);
     }
   };
   auto issue_exponents = [&](const Group &gk, const Group &gv) {  // of K's rows in lanes 0 .. 15, of V's in lanes 32 .. 47
@@ -865,10 +878,10 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
       if ((lane & 31) < (upper ? gv.have() : gk.have())) exps = *((upper ? group_exponents(p, p.v, gv) : group_exponents(p, p.k, gk)) + (lane & 31));
     }
   };
-  auto widen = [&](const u32x4_t (&from)[2], int lane0, char *to, auto place) {
+  auto widen = [&](const u32x4_t (&from)[kPieces8], int lane0, char *to, auto place) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = 8 * i + (lane >> 3), row = 16 * wave + r, granule = 2 * (lane & 7);
+    for (int i = 0; i < kPieces8; ++i) {
+      const int r = part_row + 8 * i + (lane >> 3), row = 16 * group + r, granule = 2 * (lane & 7);
       const float scale = power_of_two(__builtin_amdgcn_ds_bpermute(4 * (r + lane0), exps));
       lds_write_b128(to, place(row, granule), widen8<T>(from[i][0], from[i][1], scale));
       lds_write_b128(to, place(row, granule + 1), widen8<T>(from[i][2], from[i][3], scale));
@@ -988,7 +1001,7 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
 
   const float l_tot = pair_sum(w.l_run);
   if (t.splits > 1) {
-    const size_t slot0 = ((size_t)(t.slot + t.split) * p.Hkv + kvh) * kTileRows + 32 * wave;
+    const size_t slot0 = (((size_t)(t.slot + t.split) * p.Hkv + kvh) << p.tile_shift) + 32 * wave;
     if (w.l32 < w_rows && w.hh == 0) *reinterpret_cast<float2 *>(p.tiles.ml + (slot0 + w.l32) * 2) = float2{w.m_run * kScaleLog2e, l_tot};
     if constexpr (EIGHT) {
       // straight from the accumulators: the registers of this kernel are full (a prompt of 4096 of 28 heads, us: 150, 158 with the way below)
@@ -1042,20 +1055,21 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void tile_rows(cons
   }
 }
 
-enum PagedMode { kFewRows, kFewRuns, kTiles, kBoth };
+enum PagedMode { kFewRows, kFewRuns, kTiles, kWideTiles, kBoth };
+constexpr int threads_of(PagedMode mode) { return mode == kWideTiles ? 512 : 256; }
 
-template <typename T, bool EIGHT, PagedMode MODE> __global__ __launch_bounds__(256, 2) void paged_attn_kernel(addresses_t a, u32x4_t b, u32x2_t c, PagedAttn p) {
+template <typename T, bool EIGHT, PagedMode MODE> __global__ __launch_bounds__(threads_of(MODE), 2) void paged_attn_kernel(addresses_t a, u32x4_t b, u32x2_t c, PagedAttn p) {
   take_early(p, a, b, c);
   __shared__ __attribute__((aligned(16))) char lds[MODE == kFewRows || MODE == kFewRuns ? kFewLds : kTilesLds];
   const int unit = blockIdx.x;
   if (MODE == kFewRows || MODE == kFewRuns || (MODE == kBoth && unit < p.few_blocks))
     few_rows<T, EIGHT, MODE == kFewRuns>(p, unit, lds);
   else
-    tile_rows<T, EIGHT>(p, unit - (MODE == kBoth ? p.few_blocks : 0), lds);
+    tile_rows<T, EIGHT, threads_of(MODE) / 64>(p, unit - (MODE == kBoth ? p.few_blocks : 0), lds);
 }
 
 template <typename T> __device__ __forceinline__ void fold_row(const PagedAttn &p, const PagedTile &t, int kvh, int c, int d4) {
-  const size_t row = ((size_t)t.slot * p.Hkv + kvh) * kTileRows + c, step = (size_t)p.Hkv * kTileRows;
+  const size_t row = (((size_t)t.slot * p.Hkv + kvh) << p.tile_shift) + c, step = (size_t)p.Hkv << p.tile_shift;
   const float *po = p.tiles.o + row * kHeadDim + d4, *pml = p.tiles.ml + row * 2;
   float M = -INFINITY, L = 0.0f;
   f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
@@ -1092,15 +1106,16 @@ template <typename T> __device__ __forceinline__ void fold_row(const PagedAttn &
 }
 // Partials of a tile of a kv head, 8 rows to a workgroup, or 16 or 32 one after the other, 32 lanes of 4 dims to a row; 8 partials are on
 // their way at a time.  The more tiles the host counts with, the fewer are split, and a workgroup that finds nothing to fold costs its
-// start (us, 8 rows / 16 / 32, tiles of a kv head by the parts that run at a time: a prompt of 4096, 1.8, 135.5 / 133.3 / 133.2; six of up to 1019 of 32 kv heads, 2.7,
-// 71.5 / 70.2 / 67.4; 6 x 700 past 2000, 1.8, 100.8 / 99.1 / 100.6; 4 x 400 past 3000, 0.7, 104.9 / 102.5 / 102; 200 past 16001, 0.1, 64.9 / 67.0 / 69.2).
+// start (us, 8 rows / 16 / 32, tiles of a kv head by the parts that run at a time: a prompt of 4096, 1.8, 135.5 / 133.3 / 133.2; six of up to 1019
+// of 32 kv heads, 2.7, 71.5 / 70.2 / 67.4; 6 x 700 past 2000, 1.8, 100.8 / 99.1 / 100.6; 4 x 400 past 3000, 0.7, 104.9 / 102.5 / 102; 200 past
+// 16001, 0.1, 64.9 / 67.0 / 69.2).
 template <typename T> __global__ __launch_bounds__(256) void paged_combine_kernel(addresses_t a, u32x4_t b, u32x2_t c_, PagedAttn p) {
   take_early(p, a, b, c_);
   const int tid = threadIdx.x, lane = tid & 63, d4 = (tid & 31) * 4;
-  const int unit = (int)(blockIdx.x << p.fold_shift) / (kTileRows / 8), item = (int)fast_div(unit, p.Hkv_div), kvh = unit - item * p.Hkv;
+  const int eights = (int)(blockIdx.x << p.fold_shift), unit = eights >> (p.tile_shift - 3), item = (int)fast_div(unit, p.Hkv_div), kvh = unit - item * p.Hkv;
   PagedTile t;
   if (!find_work<false, true>(p, item, lane, t)) return;
-  const int c0 = (int)(blockIdx.x << p.fold_shift) % (kTileRows / 8) * 8, c1 = min(c0 + (8 << p.fold_shift), t.rows);
+  const int c0 = (eights * 8) & ((1 << p.tile_shift) - 1), c1 = min(c0 + (8 << p.fold_shift), t.rows);
   for (int c = c0 + (tid >> 5); c < c1; c += 8) fold_row<T>(p, t, kvh, c, d4);
 }
 
@@ -1114,15 +1129,21 @@ struct PagedPlan {
     long long folds() const { return slots / 2 < tiles ? slots / 2 : tiles; }  // tiles that are split, at most
   } few, by_tiles;
   bool runs;  // may be taken
+  bool wide;  // tiles of 256 rows, for launches without few rows
   size_t bytes(int Hkv) const { return few.bytes(Hkv) + by_tiles.bytes(Hkv); }
 };
-static PagedPlan plan_paged(int tokens, int batch, int max_q_len, int max_kv_len, int window, int sinks, int g, int Hkv) {
+// Wide tiles, 8 waves of 32 rows and one workgroup to a CU, read K and V half as often, and widen 8 bits half as often, but are half as many,
+// to be dealt to half as many places.  They are taken where rows do not fill them much worse than narrow ones, and either long caches
+// behind few tokens, which are cut into parts of about one length, are work for all places, or 8-bit prompts make rounds enough (us, narrow / wide:
+// 500 past 30000 of 28 + 4 heads 235 / 222, in 8 bits 271 / 236; 200 past 16001 65.2 / 63.8, 73.4 / 68.6; 4 x 130 past 9000 88.1 / 84.7; 100 past
+// 4000 22.7 / 26.2; prompts, whose tiles differ in length: of 2048 52.6 / 60, 65 / 66.5, of 4096 139 / 130, 153 / 135, of 6000 268 / 273, 297 / 287,
+// of 4000 of 40 + 8 177 / 183, 197 / 193).
+static PagedPlan plan_paged(int tokens, int batch, int max_q_len, int max_kv_len, int window, int sinks, int g, int Hkv, bool eight) {
   PagedPlan pl = {};
   const long long cus = device_compute_units(), sequences = batch < tokens ? batch : tokens;  // that have new tokens at all
   const bool tiles = (long long)max_q_len * g > kFewCols;
   // (all sequences have max_q_len tokens, or the tokens do not add up: no few-rows ones)
   if (!tiles || (g <= kFewCols && (long long)batch * max_q_len != tokens)) pl.few.tiles = sequences;
-  if (tiles) pl.by_tiles.tiles = (long long)tokens * g / kTileRows + sequences;
   auto deal = [&](PagedPlan::Kind &kind, int rows, int unit, long long span, long long workgroups, int least) {
     kind.rows = rows;
     kind.flags = rows == kFewCols;
@@ -1138,17 +1159,30 @@ static PagedPlan plan_paged(int tokens, int batch, int max_q_len, int max_kv_len
   };
   const long long units = deal(pl.few, kFewCols, kFewUnit, kFewCols, cus, 3);
   pl.runs = batch > 1 && batch <= 64 && pl.few.slots > 0 && pl.few.tiles * units >= (long long)kRunUnits * pl.few.parts;
-  deal(pl.by_tiles, kTileRows, kTileUnit, kTileRows / g + 1, 2 * cus, 6);
+  auto deal_tiles = [&](bool wide) {
+    const int rows = wide ? 2 * kTileRows : kTileRows;
+    pl.wide = wide;
+    if (tiles) pl.by_tiles.tiles = (long long)tokens * g / rows + sequences;
+    return deal(pl.by_tiles, rows, kTileUnit, rows / g + 1, wide ? cus : 2 * cus, 6);
+  };
+  if (tiles && !pl.few.tiles) {
+    auto filled = [&](int rows) { return ((long long)max_q_len * g + rows - 1) / rows * rows; };
+    const long long seen = deal_tiles(true), count = pl.by_tiles.tiles, parts = pl.by_tiles.parts;
+    const bool chunks = max_kv_len / 4 >= max_q_len && count * (seen / 6) >= parts, rounds = eight && window <= 0 && 2 * count >= 3 * parts;
+    if (8 * filled(2 * kTileRows) <= 9 * filled(kTileRows) && (chunks || rounds)) return pl;
+  }
+  deal_tiles(false);
   return pl;
 }
 
 size_t paged_attn_workspace_bytes(int tokens, int batch, int max_q_len, int max_kv_len, int window, int sinks, int g, int Hkv) {
-  return plan_paged(tokens, batch, max_q_len, max_kv_len, window, sinks, g, Hkv).bytes(Hkv);
+  const auto bytes = [&](bool eight) { return plan_paged(tokens, batch, max_q_len, max_kv_len, window, sinks, g, Hkv, eight).bytes(Hkv); };
+  return bytes(false) > bytes(true) ? bytes(false) : bytes(true);
 }
 
 hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, const void *v_pages, const PagedBatch &batch, void *workspace,
                              int max_q_len, int max_kv_len, int window, int sinks, int g, int Hkv, bool eight, int dt, hipStream_t stream) {
-  const PagedPlan pl = plan_paged(batch.tokens, batch.batch, max_q_len, max_kv_len, window, sinks, g, Hkv);
+  const PagedPlan pl = plan_paged(batch.tokens, batch.batch, max_q_len, max_kv_len, window, sinks, g, Hkv, eight);
   PagedAttn p = {};
   p.batch = batch;
   p.out = static_cast<char *>(out);
@@ -1175,7 +1209,9 @@ hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, cons
   p.tiles = kind_of(pl.by_tiles);
   const long long few_blocks = pl.few.items * Hkv, tile_blocks = pl.by_tiles.items * Hkv;
   p.fold_shift = pl.by_tiles.tiles > 2 * pl.by_tiles.parts ? 2 : 2 * pl.by_tiles.tiles > pl.by_tiles.parts ? 1 : 0;
-  const long long folds = pl.by_tiles.folds() * Hkv * (kTileRows / 8 >> p.fold_shift);
+  p.tile_shift = pl.wide ? 8 : 7;
+  static_assert(kTileRows == 128);
+  const long long folds = pl.by_tiles.folds() * Hkv * (1 << (p.tile_shift - 3 - p.fold_shift));
   if (pl.few.tiles + pl.by_tiles.tiles > 0x7fffffffLL || few_blocks + tile_blocks > 0x7fffffffLL || folds > 0x7fffffffLL) return hipErrorInvalidValue;
   p.number = pl.few.slots ? launch_number() : 0;
   p.few_blocks = (int)few_blocks;
@@ -1186,10 +1222,11 @@ hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, cons
   };
   const auto kern = !tile_blocks && pl.runs ? kernel_of(std::integral_constant<PagedMode, kFewRuns>())
                     : !tile_blocks ? kernel_of(std::integral_constant<PagedMode, kFewRows>())
+                    : !few_blocks && pl.wide ? kernel_of(std::integral_constant<PagedMode, kWideTiles>())
                     : !few_blocks ? kernel_of(std::integral_constant<PagedMode, kTiles>())
                                   : kernel_of(std::integral_constant<PagedMode, kBoth>());
   const PagedEarly early(p);
-  const hipError_t e = launch(kern, dim3((uint32_t)(few_blocks + tile_blocks)), 256, 0, stream, early.a, early.b, early.c, p);
+  const hipError_t e = launch(kern, dim3((uint32_t)(few_blocks + tile_blocks)), pl.wide ? 512 : 256, 0, stream, early.a, early.b, early.c, p);
   if (e != hipSuccess || folds == 0) return e;
   return launch(dt == kDtFloat16 ? paged_combine_kernel<_Float16> : paged_combine_kernel<__bf16>, dim3((uint32_t)folds), 256, 0, stream, early.a,
                 early.b, early.c, p);
