@@ -766,14 +766,14 @@ template <typename T, bool EIGHT, bool RUNS> __device__ __forceinline__ void few
 // order every later LDS read behind the loads; they are waited for where the waves meet (s_waitcnt vmcnt before a barrier).
 template <int N> __device__ __forceinline__ void load_group(u32x4_t r, const int (&o)[N], uint32_t lds_at) {
   if constexpr (N == 2)
-    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds\n\tbuffer_load_dwordx4 %1, %2, 0 offen offset:1024 lds"
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds\n\tbuffer_load_dwordx4 %1, %2, 0 offen offset:0x400 lds"
                  :
                  : "v"(o[0]), "v"(o[1]), "s"(r), "s"(lds_at)
                  : "m0", "memory");
   else
     asm volatile(
-        "s_mov_b32 m0, %5\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %4, 0 offen lds\n\tbuffer_load_dwordx4 %1, %4, 0 offen offset:1024 lds\n\t"
-        "buffer_load_dwordx4 %2, %4, 0 offen offset:2048 lds\n\tbuffer_load_dwordx4 %3, %4, 0 offen offset:3072 lds"
+        "s_mov_b32 m0, %5\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %4, 0 offen lds\n\tbuffer_load_dwordx4 %1, %4, 0 offen offset:0x400 lds\n\t"
+        "buffer_load_dwordx4 %2, %4, 0 offen offset:0x800 lds\n\tbuffer_load_dwordx4 %3, %4, 0 offen offset:0xc00 lds"
         :
         : "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3]), "s"(r), "s"(lds_at)
         : "m0", "memory");
