@@ -205,7 +205,8 @@ int llmhip_rope_kv_append(void *out_q, void *k_cache, void *v_cache, const void 
  *                                       have `tokens` rows; none, one or many.  Rows that are no sequence's are neither read nor written.
  *   kv_lens [batch]                     rows of the sequence with the new tokens: token t of sequence b is at position
  *                                       kv_lens[b] - q_starts[b + 1] + t, the last one at kv_lens[b] - 1.
- * A sequence whose rows are not all within [0, tokens), or whose length is not within [0, pages_per_seq * page_size], is passed over.
+ * A sequence whose rows are not all within [0, tokens), or whose length is not within [0, pages_per_seq * page_size], is passed over.  The
+ * others are worked on as without it, in whatever order the starts are.
  * Sequences may share pages that nobody writes; no two may append to one row, nor have one row of the dense tensors, [tokens][heads]
  * [head_dim] of dt. */
 

@@ -57,12 +57,10 @@ template <typename T> __device__ __forceinline__ void limited8(u32x4_t v, float 
 // page table to stores: 4.8 us, of which an empty launch is 1.6.
 template <typename T, bool NEOX, bool EIGHT> __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend p) {
   const int token = blockIdx.x, tid = threadIdx.x, lane = tid & 63, j = tid & 7;
-  const int b = sequence_of(p.batch, token, lane);
-  if (b >= p.batch.batch) return;
-  const int first = p.batch.q_starts[b], end = p.batch.q_starts[b + 1], len = p.batch.kv_lens[b];
-  const int pos = len - end + token;
-  if (token < first || !sequence_ok(p.batch, first, end, len) || pos < 0 || pos >= p.table_rows) return;
-  const PagePlace at = page_place(p.batch, b, pos);
+  const TokenSequence s = sequence_of(p.batch, token, lane);
+  const int pos = s.pos;
+  if (s.b < 0 || pos < 0 || pos >= p.table_rows) return;
+  const PagePlace at = page_place(p.batch, s.b, pos);
   const int rows = p.q_heads + 2 * p.kv_heads, page_rows = (int)p.batch.page_size.d;
   const float *tab = p.freq_cis + (size_t)pos * kHeadDim + (NEOX ? 16 : 8) * j;
   f32x4_t cs[4];
@@ -139,8 +137,7 @@ struct PagedRead {
 // ordinary stores 44.)
 template <typename T, bool EIGHT, int TOKENS> __global__ __launch_bounds__(256) void paged_read_kernel(PagedRead p) {
   const int token0 = blockIdx.x * TOKENS, tid = threadIdx.x, lane = tid & 63, j = tid & 15;
-  // (one token to a lane, the first TOKENS lanes)
-  const TokenPlace places = token_place(p.batch, token0, token0 + min(lane, TOKENS - 1), lane);
+  const TokenPlace places = token_places<TOKENS>(p.batch, token0, lane);
   const int page_rows = (int)p.batch.page_size.d;
   for (int r = tid >> 4; r < 2 * p.kv_heads; r += 16) {
     const bool is_v = r >= p.kv_heads;
