@@ -227,6 +227,8 @@ int llmhip_paged_rope_kv_append(void *out_q, void *k_pages, void *v_pages, const
  * Keys that a row does not see have no part in it, infinities and NaN included.
  * max_q_len: no sequence has more new tokens (one that does is passed over).  max_kv_len: no sequence is longer; if one is, the
  * call is slower and no less right.  They, tokens and batch shape the launch, and may be larger than what is there.
+ * tokens * group_size is at most 2^30, heads are at most 65535; LLMHIP_ERR_UNSUPPORTED too where these bounds ask for 2^24 workgroups or
+ * more: batch * kv_head_num (one to a sequence of few rows) and tokens * group_size * kv_head_num / 128 together.
  * workspace: llmhip_paged_flash_attn_workspace_bytes bytes for the same arguments (0 where no keys are shared among workgroups), of the
  * caller's, so that the call allocates nothing and may be captured; calls that overlap need one each.  out and q may be one buffer. */
 int llmhip_paged_flash_attn_gqa(void *out, const void *q, const void *k_pages, const void *v_pages, const int *page_table, const int *q_starts,

@@ -102,7 +102,7 @@ hipError_t launch_paged_append(void *out_q, void *k_pages, void *v_pages, const 
                                int dt, hipStream_t stream);
 hipError_t launch_paged_read(void *out_k, void *out_v, const void *k_pages, const void *v_pages, const PagedBatch &batch, int kv_heads,
                              bool eight, int dt, hipStream_t stream);
-// window 0: all keys.  A workspace of paged_attn_workspace_bytes for the same bounds.
+// window 0: all keys.  A workspace of paged_attn_workspace_bytes for the same bounds.  hipErrorNotSupported: more workgroups than a launch takes.
 size_t paged_attn_workspace_bytes(int tokens, int batch, int max_q_len, int max_kv_len, int window, int sinks, int g, int Hkv);
 hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, const void *v_pages, const PagedBatch &batch, void *workspace,
                              int max_q_len, int max_kv_len, int window, int sinks, int g, int Hkv, bool eight, int dt, hipStream_t stream);

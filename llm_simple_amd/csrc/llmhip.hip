@@ -413,8 +413,9 @@ int llmhip_paged_flash_attn_gqa(void *out, const void *q, const void *k_pages, c
   if (sinks > kMaxPagedKeys) sinks = kMaxPagedKeys;
   const size_t need = llmhip_paged_flash_attn_workspace_bytes(tokens, batch, max_q_len, max_kv_len, window, sinks, group_size, kv_head_num, head_dim);
   if (need && (!workspace || workspace_bytes < need)) return LLMHIP_ERR_WORKSPACE;
-  return from_hip(launch_paged_attn(out, q, k_pages, v_pages, b, workspace, max_q_len, max_kv_len, window, sinks, group_size, kv_head_num,
-                                    cache_dt == LLMHIP_DT_FLOAT8_E4M3, dt, as_stream(stream)));
+  const hipError_t e = launch_paged_attn(out, q, k_pages, v_pages, b, workspace, max_q_len, max_kv_len, window, sinks, group_size, kv_head_num,
+                                         cache_dt == LLMHIP_DT_FLOAT8_E4M3, dt, as_stream(stream));
+  return e == hipErrorNotSupported ? LLMHIP_ERR_UNSUPPORTED : from_hip(e);
 }
 
 /* ---------------- runtime surface ---------------- */

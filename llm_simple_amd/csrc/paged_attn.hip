@@ -1212,7 +1212,9 @@ hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, cons
   p.tile_shift = pl.wide ? 8 : 7;
   static_assert(kTileRows == 128);
   const long long folds = pl.by_tiles.folds() * Hkv * (1 << (p.tile_shift - 3 - p.fold_shift));
-  if (pl.few.tiles + pl.by_tiles.tiles > 0x7fffffffLL || few_blocks + tile_blocks > 0x7fffffffLL || folds > 0x7fffffffLL) return hipErrorInvalidValue;
+  const long long threads = pl.wide ? 512 : 256;
+  // (a launch takes fewer than 2^32 threads along a dimension)
+  if ((few_blocks + tile_blocks) * threads > 0xffffffffLL || folds * 256 > 0xffffffffLL) return hipErrorNotSupported;
   p.number = pl.few.slots ? launch_number() : 0;
   p.few_blocks = (int)few_blocks;
   auto kernel_of = [&](auto mode) {
@@ -1226,7 +1228,7 @@ hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, cons
                     : !few_blocks ? kernel_of(std::integral_constant<PagedMode, kTiles>())
                                   : kernel_of(std::integral_constant<PagedMode, kBoth>());
   const PagedEarly early(p);
-  const hipError_t e = launch(kern, dim3((uint32_t)(few_blocks + tile_blocks)), pl.wide ? 512 : 256, 0, stream, early.a, early.b, early.c, p);
+  const hipError_t e = launch(kern, dim3((uint32_t)(few_blocks + tile_blocks)), (unsigned)threads, 0, stream, early.a, early.b, early.c, p);
   if (e != hipSuccess || folds == 0) return e;
   return launch(dt == kDtFloat16 ? paged_combine_kernel<_Float16> : paged_combine_kernel<__bf16>, dim3((uint32_t)folds), 256, 0, stream, early.a,
                 early.b, early.c, p);

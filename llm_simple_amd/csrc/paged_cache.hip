@@ -20,6 +20,14 @@ namespace llmhip {
 // Rows read back: this many tokens to a workgroup from so many on, which are two workgroups to a CU (below, one: 301 tokens 2.3 us).
 constexpr int kReadTokens = 4, kManyTokens = 2048;
 
+// A launch takes fewer than 2^32 threads along a dimension: workgroup w is the one at (w % 2^20, w / 2^20) of the first and third.
+constexpr int kGridShift = 20;
+static dim3 grid_of(int workgroups, unsigned y = 1) {
+  const unsigned all = (unsigned)workgroups, most = 1u << kGridShift;
+  return all <= most ? dim3(all, y) : dim3(most, y, (all + most - 1) >> kGridShift);
+}
+__device__ __forceinline__ int workgroup() { return (int)(blockIdx.z << kGridShift | blockIdx.x); }
+
 struct PagedAppend {
   PagedBatch batch;
   char *out_q, *k_pages, *v_pages;
@@ -56,7 +64,7 @@ template <typename T> __device__ __forceinline__ void limited8(u32x4_t v, float 
 // much 16.3); several tokens to a workgroup, and rows dealt to lanes across tokens, were slower (20-23).  Few by their chain of loads, starts to
 // page table to stores: 4.8 us, of which an empty launch is 1.6.
 template <typename T, bool NEOX, bool EIGHT> __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend p) {
-  const int token = blockIdx.x, tid = threadIdx.x, lane = tid & 63, j = tid & 7;
+  const int token = workgroup(), tid = threadIdx.x, lane = tid & 63, j = tid & 7;
   const TokenSequence s = sequence_of(p.batch, token, lane);
   const int pos = s.pos;
   if (s.b < 0 || pos < 0 || pos >= p.table_rows) return;
@@ -122,7 +130,7 @@ hipError_t launch_paged_append(void *out_q, void *k_pages, void *v_pages, const 
     if (eight) return is_neox ? paged_append_kernel<T, true, true> : paged_append_kernel<T, false, true>;
     return is_neox ? paged_append_kernel<T, true, false> : paged_append_kernel<T, false, false>;
   };
-  return launch(dt == kDtFloat16 ? kernel_of(_Float16()) : kernel_of(__bf16()), dim3(batch.tokens, spread), 256, 0, stream, p);
+  return launch(dt == kDtFloat16 ? kernel_of(_Float16()) : kernel_of(__bf16()), grid_of(batch.tokens, spread), 256, 0, stream, p);
 }
 
 struct PagedRead {
@@ -136,7 +144,7 @@ struct PagedRead {
 // the memory system: 32768 rows of 8 kv heads in 8 bits, 202 MB in and out, in 39.7 us, 5.1 TB/s.  (TOKENS, us: 1 56, 2 46, 4 39.7, 8 41; with
 // ordinary stores 44.)
 template <typename T, bool EIGHT, int TOKENS> __global__ __launch_bounds__(256) void paged_read_kernel(PagedRead p) {
-  const int token0 = blockIdx.x * TOKENS, tid = threadIdx.x, lane = tid & 63, j = tid & 15;
+  const int token0 = workgroup() * TOKENS, tid = threadIdx.x, lane = tid & 63, j = tid & 15;
   const TokenPlace places = token_places<TOKENS>(p.batch, token0, lane);
   const int page_rows = (int)p.batch.page_size.d;
   for (int r = tid >> 4; r < 2 * p.kv_heads; r += 16) {
@@ -187,7 +195,7 @@ hipError_t launch_paged_read(void *out_k, void *out_v, const void *k_pages, cons
   const std::integral_constant<int, kReadTokens> some;
   const auto kern = dt == kDtFloat16 ? (many ? kernel_of(_Float16(), some) : kernel_of(_Float16(), one))
                                      : (many ? kernel_of(__bf16(), some) : kernel_of(__bf16(), one));
-  return launch(kern, dim3((batch.tokens + (many ? kReadTokens - 1 : 0)) / (many ? kReadTokens : 1)), 256, 0, stream, p);
+  return launch(kern, grid_of((batch.tokens + (many ? kReadTokens - 1 : 0)) / (many ? kReadTokens : 1)), 256, 0, stream, p);
 }
 
 }  // namespace llmhip
