@@ -224,7 +224,8 @@ int llmhip_paged_rope_kv_append(void *out_q, void *k_pages, void *v_pages, const
 /* Attention of the new tokens, which llmhip_paged_rope_kv_append has put into the pages before: of one token to a sequence (decode), pieces of
  * prompts, whole prompts, all of these in one batch.  Query head h reads kv head h / group_size.  A token at position p sees key c if
  * c <= p and, with window > 0, c > p - window or c < sinks; window <= 0: all keys up to p.  A row that sees no key is zeros.
- * Keys that a row does not see have no part in it, infinities and NaN included.
+ * Keys that a row does not see have no part in it, infinities and NaN included; a V that is not finite makes the same dims of the rows
+ * that see it not finite, and no others.
  * max_q_len: no sequence has more new tokens (one that does is passed over).  max_kv_len: no sequence is longer; if one is, the
  * call is slower and no less right.  They, tokens and batch shape the launch, and may be larger than what is there.
  * tokens * group_size is at most 2^30, heads are at most 65535; LLMHIP_ERR_UNSUPPORTED too where these bounds ask for 2^24 workgroups or

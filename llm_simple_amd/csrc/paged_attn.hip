@@ -28,8 +28,8 @@
 //
 // Keys that a row must not see: their scores become -inf, so their K does not matter, but a weight of 0 times a V that is not finite
 // would be NaN.  Rows behind the last key, and pages that are not there, are zeros (the loads' descriptors end before them).  V of keys
-// that only some rows see is what it is: a row whose result is not finite is computed again key by key (exact_row), from the
-// keys that it sees alone.
+// that only some rows see is what it is: a wave that finds a row of its own not finite in the end goes over its keys once more
+// (rows_again), and adds up those 32 of which a row must not see one key by key, from what each row sees.
 #include <type_traits>
 
 #include "common.hpp"
@@ -378,73 +378,129 @@ __device__ __forceinline__ bool sees(const PagedAttn &p, int pos, int key) {
   return key <= pos && (p.window <= 0 || key > pos - p.window || key < p.sinks);
 }
 
-// One row by G lanes, from the keys that it sees alone; see the header.  Lane i has 128 / G dims from 128 / G * i on.  M is in units of
-// score times log2 e.
-template <typename T, bool EIGHT, int G, int UNIT>
-__device__ __forceinline__ void exact_row(const PagedAttn &p, int b, int kvh, const char *q_row, int pos, PagedKeys keys, int u0, int u1, float &M,
-                                          float &L, float (&o)[kHeadDim / G]) {
-  constexpr int D = kHeadDim / G, W = cached_row_bytes(EIGHT);
-  const int lane = threadIdx.x & (G - 1);
+// The lane, and the kernels' arguments, of which the compiler has computed or loaded nothing before: code that hardly runs keeps nothing in
+// registers elsewhere.
+__device__ __forceinline__ int fresh_lane() {
+  int none = 0;
+  asm volatile("" : "+v"(none));
+  return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, (uint32_t)none));
+}
+struct PagedArguments {  // as the kernels have them
+  addresses_t a;
+  u32x4_t b;
+  u32x2_t c;
+  PagedAttn p;
+};
+__device__ __forceinline__ PagedAttn fresh_arguments() {
+  typedef __attribute__((address_space(4))) const PagedArguments Constant;
+  uint64_t at = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  PagedAttn p;
+  __builtin_memcpy(&p, (const void *)&((Constant *)at)->p, sizeof(p));
+  return p;
+}
+
+// The 32 rows of a wave (w.qf, at positions pos) over keys first .. first + 31 of every `step` of the part's units, once more and by the wave alone; see
+// the header.  32 keys at a time, K and then V through `mine`, 8 KiB of the wave's own.  Where a row must not see one of the keys that are there,
+// the product goes key by key, a key's V for the rows that see it.  The reference of the weights is the running maximum itself: a sum that only
+// its slack made too large for 32 bits is none here.
+//
+// Nothing of this is on the way of rows that are finite, and no row, nor any number of such V, makes a call more than some times longer (us of 28 + 4
+// heads, without / with a NaN in one dim of the first key / row by row and key by key as the only way: a prompt of 1024 31 / 90 / 3700, of 4096 152 / 740 /
+// 30000, 200 past 16001 67 / 290 / 12400, 3 past 2000 17 / 51 / 1900).
+template <typename T, bool EIGHT, int UNIT>
+__device__ __forceinline__ void rows_again(int b, int kvh, WaveAttn<T, 1> &w, int pos, const PagedKeys &keys, int u0, int u1,
+                                           int first, int step, char *mine) {
+  constexpr int W = cached_row_bytes(EIGHT), kLoads = EIGHT ? 4 : 8;  // bytes of a row; loads of a lane, which has half of one
+  const PagedAttn p = fresh_arguments();
+  int lane = fresh_lane(), r = lane >> 1, half = lane & 1;
   const size_t exponents = (size_t)p.Hkv * p.batch.page_size.d * kHeadDim;
-  M = -INFINITY;
-  L = 0.0f;
+  w.init(mine, lane, 0);
+  f32x16_t s[1];
+  auto stage = [&](const u32x4_t (&x)[kLoads], int byte, auto place) {
 #pragma unroll
-  for (int d = 0; d < D; ++d) o[d] = 0.0f;
-  for (int u = u0; u < u1; ++u)
-    for (int k0 = 0; k0 < UNIT; k0 += G) {
-      const int key = keys.base(u, UNIT) + k0 + lane;
-      PagePlace at = {-1, 0};
-      if (key < keys.limit(u) && sees(p, pos, key)) at = page_place(p.batch, b, key);
-      const bool visible = at.there(p.batch);
-      const int64_t page_at = visible ? (int64_t)at.page * p.batch.page_stride : 0;
-      const int row = visible ? kvh * (int)p.batch.page_size.d + at.row : 0;
-      float s = -INFINITY;
-      if (visible) {
-        const char *k_row = p.k + page_at + (size_t)row * W;
-        const float scale = EIGHT ? power_of_two((uint8_t)p.k[page_at + exponents + row]) : 1.0f;
-        s = 0.0f;
-        for (int c = 0; c < kHeadDim; c += 8) {
-          const u32x4_t qv = global_load_b128(q_row + c * 2);
-          u32x4_t kv;
-          if constexpr (EIGHT) {
-            const u32x2_t w = *reinterpret_cast<const u32x2_t *>(k_row + c);
-            kv = widen8<T>(w[0], w[1], scale);
-          } else {
-            kv = global_load_b128(k_row + c * 2);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            s += Elem<T>::widen((uint16_t)(qv[i >> 1] >> ((i & 1) * 16))) * Elem<T>::widen((uint16_t)(kv[i >> 1] >> ((i & 1) * 16)));
-        }
-        s *= kScaleLog2e;
-      }
-      float most = s;
-      for (int x = 1; x < G; x *= 2) most = fmaxf(most, __shfl_xor(most, x, G));
-      const float m_new = fmaxf(M, most), m_use = m_new == -INFINITY ? 0.0f : m_new;
-      const float alpha = fast_exp2(M - m_use), weight = visible ? fast_exp2(s - m_use) : 0.0f;
-      M = m_new;
-      L = L * alpha + weight;
-#pragma unroll
-      for (int d = 0; d < D; ++d) o[d] *= alpha;
-      for (int i = 0; i < G; ++i) {
-        const float w = __shfl(weight, i, G);
-        const int at_page = __shfl(visible ? at.page : -1, i, G), at_row = __shfl(row, i, G);
-        if (at_page < 0) continue;
-        const char *v_row = p.v + (int64_t)at_page * p.batch.page_stride + (size_t)at_row * W;
-        const float scale = EIGHT ? power_of_two((uint8_t)p.v[(int64_t)at_page * p.batch.page_stride + exponents + at_row]) : 1.0f;
-#pragma unroll
-        for (int d = 0; d < D; d += 2) {
-          uint32_t pair;
-          if constexpr (EIGHT)
-            pair = widen_pair<T, false>(*reinterpret_cast<const uint16_t *>(v_row + D * lane + d), scale);
-          else
-            pair = *reinterpret_cast<const uint32_t *>(v_row + (D * lane + d) * 2);
-          o[d] += w * Elem<T>::widen((uint16_t)pair);
-          o[d + 1] += w * Elem<T>::widen((uint16_t)(pair >> 16));
-        }
+    for (int c = 0; c < kLoads; ++c) {
+      if constexpr (EIGHT) {
+        const float scale = power_of_two(byte);
+        lds_write_b128(mine, place(r, 8 * half + 2 * c), widen8<T>(x[c][0], x[c][1], scale));
+        lds_write_b128(mine, place(r, 8 * half + 2 * c + 1), widen8<T>(x[c][2], x[c][3], scale));
+      } else {
+        lds_write_b128(mine, place(r, 8 * half + c), x[c]);
       }
     }
-  for (int x = 1; x < G; x *= 2) L += __shfl_xor(L, x, G);
+  };
+#pragma unroll 1
+  for (int u = u0; u < u1; ++u)
+#pragma unroll 1
+    for (int k0 = first; k0 < UNIT; k0 += step) {
+      asm volatile("" : "+v"(r), "+v"(half));  // (the places in LDS worked out anew: registers)
+      const int base = keys.base(u, UNIT) + k0, limit = keys.limit(u);
+      PagePlace at = {-1, 0};
+      if (base + r < limit) at = page_place(p.batch, b, base + r);
+      const bool there = at.there(p.batch);
+      const uint64_t rows_there = __builtin_amdgcn_ballot_w64(there);
+      if (rows_there == 0) continue;
+      const int64_t page_at = there ? (int64_t)at.page * p.batch.page_stride : 0;
+      const uint32_t row = (uint32_t)(kvh * (int)p.batch.page_size.d + at.row);
+      auto fetch = [&](const char *pool, u32x4_t (&x)[kLoads], int &byte) {
+        byte = 127;
+#pragma unroll
+        for (int c = 0; c < kLoads; ++c) x[c] = u32x4_t{};
+        if (!there) return;
+        const char *page = pool + page_at;
+#pragma unroll
+        for (int c = 0; c < kLoads; ++c) x[c] = global_load_b128(page + (size_t)row * W + half * (W / 2) + c * 16);
+        if constexpr (EIGHT) byte = (uint8_t)page[exponents + row];
+      };
+      u32x4_t x[kLoads];
+      int byte;
+      fetch(p.k, x, byte);
+      __builtin_amdgcn_wave_barrier();
+      stage(x, byte, [](int row, int granule) { return k_swizzle_off(row, granule); });
+      __builtin_amdgcn_wave_barrier();
+      fetch(p.v, x, byte);
+      w.qk(mine, 0, s);
+      __builtin_amdgcn_wave_barrier();
+      stage(x, byte, [](int row, int granule) { return v_swizzle_off(row, granule); });
+      __builtin_amdgcn_wave_barrier();
+      const uint64_t mine_there = rows_there >> (8 * w.hh);
+      bool some_hidden = false;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int c = 8 * (i >> 2) + (i & 3);
+        const bool is_there = mine_there >> (2 * c) & 1, seen = sees(p, pos, base + 4 * w.hh + c);
+        some_hidden |= is_there && !seen;
+        s[0][i] = is_there && seen ? s[0][i] : -INFINITY;
+      }
+      w.template row_max<false>(s, kScaleLog2e);
+      w.l_run += w.probabilities(s, kScaleLog2e);
+      if (__builtin_amdgcn_ballot_w64(some_hidden) == 0) {
+        w.pv(0);
+        continue;
+      }
+#pragma unroll 1
+      for (int key = 0; key < 32; ++key) {
+        const int i = 4 * (key >> 3) + (key & 3);  // element of the half key >> 2 & 1 of the lanes
+        uint32_t pair = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pair = j == i >> 1 ? w.pf[0][j >> 2][j & 3] : pair;
+        pair = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (w.l32 + 8 * (key & 4)), (int)pair);
+        const float weight = Elem<T>::widen((uint16_t)(i & 1 ? pair >> 16 : pair));
+        const bool seen = sees(p, pos, base + key);
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            const u32x2_t x = *reinterpret_cast<const u32x2_t *>(mine + v_swizzle_off(key, 4 * d + i4) + w.hh * 8);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float o = w.o[d][4 * i4 + j];
+              const float more = __builtin_fmaf(weight, Elem<T>::widen((uint16_t)(x[j >> 1] >> ((j & 1) * 16))), o);
+              w.o[d][4 * i4 + j] = seen ? more : o;
+            }
+          }
+      }
+    }
 }
 
 // ---- few rows ----
@@ -458,7 +514,7 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows_of(co
   // steps on their way, as many bytes (16 x 32768, through LDS 175 / 169, one step 190; 48 ragged 120 / 107).
   constexpr bool kStaged = !EIGHT;
   constexpr int kAhead = EIGHT ? 2 : 1;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, cg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = fresh_lane(), tid = wave * 64 + lane, col = lane & 15, cg = lane >> 4;
   const int p0 = t.len - t.m, p1 = t.len - 1;
   const PagedKeys keys = keys_seen<kFewUnit>(p, p0, p1, t.len);
   const PagedPart part = part_of(t, keys.units);
@@ -622,6 +678,39 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows_of(co
     }
     if (kAhead > 1 && it < iters) step(a, it);
   }
+  // Rows that are not finite, where some see keys that others do not
+  if (t.m > 1 || p.window > 0) {
+    float size = 0.0f;
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) size += __builtin_fabsf(o[d][i]);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(size < INFINITY)) != 0, 0)) {
+      WaveAttn<T, 1> w;
+      const int l = fresh_lane(), row = min(l & 31, t.rows - 1), tok = (int)fast_div(row, p.g_div);
+      const char *qp = p.q + ((size_t)(t.start + tok) * p.H + kvh * p.g + row - tok * p.g) * kRowBytes + (l >> 5) * 16;
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) w.qf[kk] = global_load_b128(qp + kk * 32);
+      rows_again<T, EIGHT, kFewUnit>(t.b, kvh, w, p0 + tok, keys, part.u0, part.u1, 32 * wave, kFewUnit, vl);
+      // from its columns to those here, through LDS as below
+      float *rows = reinterpret_cast<float *>(vl);
+      __builtin_amdgcn_wave_barrier();
+      if (w.l32 < kFewCols) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4)
+            *reinterpret_cast<f32x4_t *>(rows + w.l32 * kHeadDim + (((8 * d + 2 * i4 + w.hh) ^ w.l32) << 2)) =
+                f32x4_t{w.o[d][4 * i4], w.o[d][4 * i4 + 1], w.o[d][4 * i4 + 2], w.o[d][4 * i4 + 3]};
+      }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int d = 0; d < 8; ++d) o[d] = *reinterpret_cast<const f32x4_t *>(rows + (l & 15) * kHeadDim + (((4 * d + (l >> 4)) ^ (l & 15)) << 2));
+      m_run = __shfl(w.m_run * kScaleLog2e, l & 15, 64);
+      l_run = __shfl(pair_sum(w.l_run), l & 15, 64);
+      if (l >> 4 != 0) l_run = 0.0f;
+    }
+  }
 
   // ---- merge the waves: [wave][col][128], the pieces of a row XORed with the column ----
   const float l_tot = quad_sum(l_run);
@@ -666,12 +755,6 @@ template <typename T, bool EIGHT> __device__ __forceinline__ void few_rows_of(co
         acc[4 + j] += wt * s1[j];
       }
     }
-    float size = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) size += __builtin_fabsf(acc[j]);
-    const bool finite = size < INFINITY;
-    if (__builtin_expect(((__builtin_amdgcn_ballot_w64(!finite) >> (lane & 48)) & 0xffff) != 0, 0))
-      exact_row<T, EIGHT, 16, kFewUnit>(p, t.b, kvh, p.q + row_at, p0 + tok, keys, part.u0, part.u1, M, L, acc);
     if (t.splits == 1) {
       store_row();
     } else {
@@ -952,8 +1035,12 @@ template <typename T, bool EIGHT, int WAVES> __device__ __forceinline__ void til
       w.template qk<0, 3>(lds, next, s_next);
       w.row_max(s, scale);
       w.template qk<3, 8>(lds, next, s_next);
-      w.l_run += w.probabilities(s, scale);
-      w.pv(slot * kUnitBytes);
+      if constexpr (EIGHT) {
+        w.l_run += w.probabilities_and_pv(s, scale, slot * kUnitBytes);
+      } else {
+        w.l_run += w.probabilities(s, scale);
+        w.pv(slot * kUnitBytes);
+      }
     }
     widen_k(slot);
     widen_v(slot ^ 1);
@@ -971,31 +1058,25 @@ template <typename T, bool EIGHT, int WAVES> __device__ __forceinline__ void til
     if (it + 1 < iters) step(it + 1, std::integral_constant<int, 1>(), sb, sa);
   }
 
-  // ---- rows that are not finite, key by key ----
+  // ---- rows that are not finite, once more ----
   char *mine = lds + wave * 32 * kRowBytes;
   float size = 0.0f;
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) size += __builtin_fabsf(w.o[d][i]);
-  uint64_t bad = __builtin_amdgcn_ballot_w64(!(size < INFINITY));
-  for (uint32_t rows = (uint32_t)(bad | bad >> 32); __builtin_expect(rows != 0, 0); rows &= rows - 1) {
-    const int r = __builtin_ctz(rows);
-    if (r >= w_rows) break;
-    float M, L, x[2];
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(size < INFINITY)) != 0 && w_rows > 0, 0)) {
+    WaveAttn<T, 1> again;
+    const int l = fresh_lane();
     int tok;
-    const char *q_row = p.q + place_of(r, tok);
-    exact_row<T, EIGHT, 64, kTileUnit>(p, t.b, kvh, q_row, before + tok, keys, part.u0, part.u1, M, L, x);
-    *reinterpret_cast<float2 *>(mine + lane * 8) = float2{x[0], x[1]};
-    __builtin_amdgcn_wave_barrier();
-    if (w.l32 == r) {
+    const char *qp = p.q + place_of(min(l & 31, w_rows - 1), tok) + (l >> 5) * 16;
 #pragma unroll
-      for (int d = 0; d < 4; ++d)
+    for (int kk = 0; kk < 8; ++kk) again.qf[kk] = global_load_b128(qp + kk * 32);
+    rows_again<T, EIGHT, kTileUnit>(t.b, kvh, again, before + tok, keys, part.u0, part.u1, 0, 32, mine);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w.o[d][i] = *reinterpret_cast<const float *>(mine + (32 * d + 8 * (i >> 2) + 4 * w.hh + (i & 3)) * 4);
-      w.m_run = M / kScaleLog2e;
-      w.l_run = w.hh == 0 ? L : 0.0f;
-    }
+    for (int d = 0; d < 4; ++d) w.o[d] = again.o[d];
+    w.m_run = again.m_run;
+    w.l_run = again.l_run;
     __builtin_amdgcn_wave_barrier();
   }
 

@@ -114,12 +114,12 @@ template <typename T, int KB = 2> struct WaveAttn {
     });
   }
 
-  // O^T += V^T P^T over the V tile at byte offset `voff` past the start of the V region.
+  // O^T += V^T P^T over the V tile at byte offset `voff` past the start of the V region, pieces I0 .. I1 - 1 of 16 keys.
   // Lane (d = 32*dblk + l32, hh): element e of k-step (kb, ks2) is the key
   // 32*kb + 16*ks2 + 8*(e/4) + 4*hh + e%4 -- the key P's element e carries.
-  template <typename Hook = NoHook>
+  template <int I0 = 0, int I1 = 2 * KB, typename Hook = NoHook>
   __device__ __forceinline__ void pv(int voff, Hook hook = Hook()) {
-    static_for<0, 8 * KB>([&](auto i_) {
+    static_for<4 * I0, 4 * I1>([&](auto i_) {
       constexpr int i = decltype(i_)::value, kb = i / 8, ks2 = i / 4 % 2, d = i % 4;
       const int c = voff + (kb * 32 + ks2 * 16) * kRowBytes;
       const u32x2_t lo = lds_read_tr16(v_addr[d], c);
@@ -171,14 +171,43 @@ template <typename T, int KB = 2> struct WaveAttn {
     return ps0 + ps1;
   }
 
+  // probabilities() and pv() in one, the exponentials between the matrix instructions, in the order they are to be issued: for kernels whose
+  // registers are so full that the compiler leaves the order as it is.  The first five quarters of a piece of 16 keys go before, then one to a
+  // matrix instruction (8-bit tiles over pages, us, all before / 4 / 5 / 6 quarters: a prompt of 2048 tokens of 28 + 4 heads 68.5 / 66.0 / 63.7 / 69.1,
+  // 8192 with a window of 1024 176 / 169 / 165 / 177; and in qk's place, from its third fragment on, 67-70 and 171-178).
+  __device__ __forceinline__ float probabilities_and_pv(const f32x16_t (&s)[KB], float c, int voff) {
+    constexpr int kAhead = 5;
+    float ps0 = 0.0f, ps1 = 0.0f;
+    auto quarter = [&](auto j_) {  // of the four pairs of each piece
+      constexpr int j = decltype(j_)::value, kb = j / 8, ks2 = j / 4 % 2, e2 = j % 4;
+      const float e0 = fast_exp2(__builtin_fmaf(s[kb][8 * ks2 + 2 * e2], c, neg_ms));
+      const float e1 = fast_exp2(__builtin_fmaf(s[kb][8 * ks2 + 2 * e2 + 1], c, neg_ms));
+      const uint32_t w = E::pack2(e0, e1);
+      pf[kb][ks2][e2] = w;
+      if (e2 & 1)
+        ps1 = dot2_ones<T>(w, ps1);
+      else
+        ps0 = dot2_ones<T>(w, ps0);
+    };
+    static_for<0, kAhead>(quarter);
+    static_for<0, 2 * KB>([&](auto i_) {
+      constexpr int i = decltype(i_)::value;
+      pv<i, i + 1>(voff, [&](auto j_) {
+        constexpr int j = decltype(j_)::value + kAhead;
+        if constexpr (j < 8 * KB) quarter(std::integral_constant<int, j>());
+      });
+    });
+    return ps0 + ps1;
+  }
+
   // First half of the online softmax of one tile of (already masked) scores: row maxima and,
   // rarely, the move of the reference.  m_run is the reference maximum used in the exponent,
   // in raw score units.  It moves only when a row maximum exceeds it by more than kLazyLog2
   // in log2 units (probabilities then stay below 2^kLazyLog2, harmless in fp32 sums and in
   // the 16-bit P operand); a -inf reference always moves.  O and l are rescaled only then,
   // which after the first tiles is rare: what depends on the reference alone (the line `move_above`, the additive term
-  // of the exponent) is computed then too, and a lane pair compares notes only then.
-  __device__ __forceinline__ void row_max(const f32x16_t (&s)[KB], float scale_log2e) {
+  // of the exponent) is computed then too, and a lane pair compares notes only then.  LAZY false: it moves with every new maximum.
+  template <bool LAZY = true> __device__ __forceinline__ void row_max(const f32x16_t (&s)[KB], float scale_log2e) {
     float m0 = -INFINITY, m1 = -INFINITY;  // two chains: half the dependent latency
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -204,7 +233,7 @@ template <typename T, int KB = 2> struct WaveAttn {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
       m_run = m_new;
-      move_above = m_new + kLazyLog2 / scale_log2e;
+      move_above = LAZY ? m_new + kLazyLog2 / scale_log2e : m_new;
       neg_ms = -m_use * scale_log2e;
     }
   }
