@@ -54,6 +54,11 @@ int llmhip_bench_matmul_alone(void *out, const void *lhs, const void *weight, co
 /* The tile by which llmhip_matmul(_bias) of 17 rows or more goes where k is not cut, lhs rows << 16 | features; 0: not by tiles. */
 int llmhip_bench_matmul_tile(int m, int n, int k);
 
+/* The kernel by which llmhip_paged_flash_attn_gqa goes with these bounds.  0: few rows (at most 16 to a sequence), equal parts; 1: few rows, in runs
+ * over all sequences where their lengths ask for it; 2: tiles of 128 rows; 3: of 256; 4: few rows and tiles of 128. */
+int llmhip_bench_paged_attn_kind(int tokens, int batch, int max_q_len, int max_kv_len, int window, int sinks, int group_size, int kv_head_num,
+                                 int eight_bits);
+
 /* Runs, for about target_ms (<= 2000), a loop of back-to-back bf16 32x32x16 MFMAs on N(0,1)
  * operands on every CU and returns the sustained TFLOP/s.  mix 0: the MFMAs alone (what the matrix
  * pipe sustains at the clock its own power draw allows); mix 1: the same MFMAs with the LDS

@@ -7,6 +7,7 @@
 
 #include "bench_kernels.hpp"
 #include "kernels.hpp"
+#include "paged_plan.hpp"
 
 using namespace LLMHIP_NS;
 
@@ -101,6 +102,12 @@ int llmhip_bench_matmul_alone(void *out, const void *lhs, const void *weight, co
   if (device_count() < 1) return LLMHIP_ERR_NO_DEVICE;
   return from_hip(launch_matmul_tile(out, lhs, weight, static_cast<const float *>(bias_f32), m, n, k, dt, static_cast<hipStream_t>(stream),
                                      pieces, workspace));
+}
+
+int llmhip_bench_paged_attn_kind(int tokens, int batch, int max_q_len, int max_kv_len, int window, int sinks, int group_size, int kv_head_num,
+                                 int eight_bits) {
+  if (tokens < 1 || batch < 1 || max_q_len < 1 || max_kv_len < 0 || sinks < 0 || group_size < 1 || kv_head_num < 1) return LLMHIP_ERR_INVALID_ARG;
+  return plan_paged(tokens, batch, max_q_len, max_kv_len, window > 0 ? window : 0, sinks, group_size, kv_head_num, eight_bits != 0).mode();
 }
 
 int llmhip_bench_matmul_tile(int m, int n, int k) { return m < 1 || n < 1 || k < 1 ? LLMHIP_ERR_INVALID_ARG : matmul_tile_size(m, n, k); }

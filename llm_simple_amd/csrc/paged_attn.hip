@@ -36,15 +36,11 @@
 #include "kernels.hpp"
 #include "lanes.hpp"
 #include "paged.hpp"
+#include "paged_plan.hpp"
 #include "wave_attn.hpp"
 
 namespace llmhip {
 
-constexpr int kFewCols = 16;     // rows of a few-rows workgroup
-constexpr int kFlagBytes = 16;   // place of a flag (few_rows_of)
-constexpr int kFewUnit = 128;    // keys of a unit, 32 to a wave
-constexpr int kTileRows = 128;   // rows of a tile (wide: twice as many)
-constexpr int kTileUnit = 64;    // keys of a unit
 constexpr int kUnitBytes = kTileUnit * kRowBytes;
 constexpr int kWaveStage = 32 * kRowBytes;  // staging of a few-rows wave, for K and for V
 constexpr int kFewLds = 8 * kWaveStage, kTilesLds = 4 * kUnitBytes;
@@ -202,7 +198,6 @@ template <bool FEW, bool FOLD> __device__ __forceinline__ bool find_alone(const 
 // costs the start of another.  (us, parts / runs: 48 sequences of up to 16384 keys of 4 kv heads, 48 units to a run, 16 bits 167 / 145, 8 bits 107 /
 // 85; 24 of up to 8192 of 8, 24 units, 76.7 / 72.2 and 52.4 / 51.4; with a window of 4096, 20 units, 61.2 / 67.0; 64 of up to 2048 of 2, 4 units,
 // 19.9 / 23.2.)  A kernel of its own, for bounds that allow runs: the loop over sequences costs a call of 7 us 0.6.
-constexpr int kRunUnits = 24;
 struct FewRuns {
   PagedSeqs<true> s;
   int units, upto, slot;  // of a lane's sequence: units, those up to its end, its first partial's slot
@@ -1136,9 +1131,6 @@ template <typename T, bool EIGHT, int WAVES> __device__ __forceinline__ void til
   }
 }
 
-enum PagedMode { kFewRows, kFewRuns, kTiles, kWideTiles, kBoth };
-constexpr int threads_of(PagedMode mode) { return mode == kWideTiles ? 512 : 256; }
-
 template <typename T, bool EIGHT, PagedMode MODE> __global__ __launch_bounds__(threads_of(MODE), 2) void paged_attn_kernel(addresses_t a, u32x4_t b, u32x2_t c, PagedAttn p) {
   take_early(p, a, b, c);
   __shared__ __attribute__((aligned(16))) char lds[MODE == kFewRows || MODE == kFewRuns ? kFewLds : kTilesLds];
@@ -1200,62 +1192,6 @@ template <typename T> __global__ __launch_bounds__(256) void paged_combine_kerne
   for (int c = c0 + (tid >> 5); c < c1; c += 8) fold_row<T>(p, t, kvh, c, d4);
 }
 
-// How a launch is shaped, from what the host knows: bounds, not lengths.
-struct PagedPlan {
-  struct Kind {
-    long long tiles, items, slots, rows;  // at most; rows of a partial
-    int least, parts;
-    bool flags;
-    size_t bytes(int Hkv) const { return (size_t)slots * Hkv * (rows * (kHeadDim + 2) * sizeof(float) + (flags ? kFlagBytes : 0)); }
-    long long folds() const { return slots / 2 < tiles ? slots / 2 : tiles; }  // tiles that are split, at most
-  } few, by_tiles;
-  bool runs;  // may be taken
-  bool wide;  // tiles of 256 rows, for launches without few rows
-  size_t bytes(int Hkv) const { return few.bytes(Hkv) + by_tiles.bytes(Hkv); }
-};
-// Wide tiles, 8 waves of 32 rows and one workgroup to a CU, read K and V half as often, and widen 8 bits half as often, but are half as many,
-// to be dealt to half as many places.  They are taken where rows do not fill them much worse than narrow ones, and either long caches
-// behind few tokens, which are cut into parts of about one length, are work for all places, or 8-bit prompts make rounds enough (us, narrow / wide:
-// 500 past 30000 of 28 + 4 heads 235 / 222, in 8 bits 271 / 236; 200 past 16001 65.2 / 63.8, 73.4 / 68.6; 4 x 130 past 9000 88.1 / 84.7; 100 past
-// 4000 22.7 / 26.2; prompts, whose tiles differ in length: of 2048 52.6 / 60, 65 / 66.5, of 4096 139 / 130, 153 / 135, of 6000 268 / 273, 297 / 287,
-// of 4000 of 40 + 8 177 / 183, 197 / 193).
-static PagedPlan plan_paged(int tokens, int batch, int max_q_len, int max_kv_len, int window, int sinks, int g, int Hkv, bool eight) {
-  PagedPlan pl = {};
-  const long long cus = device_compute_units(), sequences = batch < tokens ? batch : tokens;  // that have new tokens at all
-  const bool tiles = (long long)max_q_len * g > kFewCols;
-  // (all sequences have max_q_len tokens, or the tokens do not add up: no few-rows ones)
-  if (!tiles || (g <= kFewCols && (long long)batch * max_q_len != tokens)) pl.few.tiles = sequences;
-  auto deal = [&](PagedPlan::Kind &kind, int rows, int unit, long long span, long long workgroups, int least) {
-    kind.rows = rows;
-    kind.flags = rows == kFewCols;
-    kind.least = least;
-    kind.parts = Hkv <= workgroups ? (int)(workgroups / Hkv) : 1;
-    const long long windowed = (long long)window + span + sinks + 2 * kPageGroup, seen = window > 0 && windowed < max_kv_len ? windowed : max_kv_len;
-    const long long units = (seen + unit - 1) / unit, all = (long long)kind.parts + 1 + kind.parts / 64;
-    kind.slots = kind.tiles > 0 && units > least && Hkv <= workgroups ? 2 * all : 0;
-    const long long most = kind.tiles * (units / least + 1);
-    if (kind.slots > most) kind.slots = most;
-    kind.items = kind.tiles + (kind.slots ? all : 0);
-    return units;
-  };
-  const long long units = deal(pl.few, kFewCols, kFewUnit, kFewCols, cus, 3);
-  pl.runs = batch > 1 && batch <= 64 && pl.few.slots > 0 && pl.few.tiles * units >= (long long)kRunUnits * pl.few.parts;
-  auto deal_tiles = [&](bool wide) {
-    const int rows = wide ? 2 * kTileRows : kTileRows;
-    pl.wide = wide;
-    if (tiles) pl.by_tiles.tiles = (long long)tokens * g / rows + sequences;
-    return deal(pl.by_tiles, rows, kTileUnit, rows / g + 1, wide ? cus : 2 * cus, 6);
-  };
-  if (tiles && !pl.few.tiles) {
-    auto filled = [&](int rows) { return ((long long)max_q_len * g + rows - 1) / rows * rows; };
-    const long long seen = deal_tiles(true), count = pl.by_tiles.tiles, parts = pl.by_tiles.parts;
-    const bool chunks = max_kv_len / 4 >= max_q_len && count * (seen / 6) >= parts, rounds = eight && window <= 0 && 2 * count >= 3 * parts;
-    if (8 * filled(2 * kTileRows) <= 9 * filled(kTileRows) && (chunks || rounds)) return pl;
-  }
-  deal_tiles(false);
-  return pl;
-}
-
 size_t paged_attn_workspace_bytes(int tokens, int batch, int max_q_len, int max_kv_len, int window, int sinks, int g, int Hkv) {
   const auto bytes = [&](bool eight) { return plan_paged(tokens, batch, max_q_len, max_kv_len, window, sinks, g, Hkv, eight).bytes(Hkv); };
   return bytes(false) > bytes(true) ? bytes(false) : bytes(true);
@@ -1293,7 +1229,7 @@ hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, cons
   p.tile_shift = pl.wide ? 8 : 7;
   static_assert(kTileRows == 128);
   const long long folds = pl.by_tiles.folds() * Hkv * (1 << (p.tile_shift - 3 - p.fold_shift));
-  const long long threads = pl.wide ? 512 : 256;
+  const long long threads = threads_of(pl.mode());
   // (a launch takes fewer than 2^32 threads along a dimension)
   if ((few_blocks + tile_blocks) * threads > 0xffffffffLL || folds * 256 > 0xffffffffLL) return hipErrorNotSupported;
   p.number = pl.few.slots ? launch_number() : 0;
@@ -1303,11 +1239,14 @@ hipError_t launch_paged_attn(void *out, const void *q, const void *k_pages, cons
     if (dt == kDtFloat16) return eight ? paged_attn_kernel<_Float16, true, MODE> : paged_attn_kernel<_Float16, false, MODE>;
     return eight ? paged_attn_kernel<__bf16, true, MODE> : paged_attn_kernel<__bf16, false, MODE>;
   };
-  const auto kern = !tile_blocks && pl.runs ? kernel_of(std::integral_constant<PagedMode, kFewRuns>())
-                    : !tile_blocks ? kernel_of(std::integral_constant<PagedMode, kFewRows>())
-                    : !few_blocks && pl.wide ? kernel_of(std::integral_constant<PagedMode, kWideTiles>())
-                    : !few_blocks ? kernel_of(std::integral_constant<PagedMode, kTiles>())
-                                  : kernel_of(std::integral_constant<PagedMode, kBoth>());
+  auto kern = kernel_of(std::integral_constant<PagedMode, kBoth>());
+  switch (pl.mode()) {
+    case kFewRows: kern = kernel_of(std::integral_constant<PagedMode, kFewRows>()); break;
+    case kFewRuns: kern = kernel_of(std::integral_constant<PagedMode, kFewRuns>()); break;
+    case kTiles: kern = kernel_of(std::integral_constant<PagedMode, kTiles>()); break;
+    case kWideTiles: kern = kernel_of(std::integral_constant<PagedMode, kWideTiles>()); break;
+    case kBoth: break;
+  }
   const PagedEarly early(p);
   const hipError_t e = launch(kern, dim3((uint32_t)(few_blocks + tile_blocks)), (unsigned)threads, 0, stream, early.a, early.b, early.c, p);
   if (e != hipSuccess || folds == 0) return e;
