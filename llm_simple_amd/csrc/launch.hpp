@@ -43,6 +43,8 @@ inline hipFunction_t function_of(const void *kern, hipStream_t stream) {
 // hipGetLastError only: 2.91 us of the host a launch, 2.70 so.
 template <typename... P, typename... A>
 inline hipError_t launch(void (*kern)(P...), dim3 grid, unsigned threads, size_t lds_bytes, hipStream_t stream, const A &...given) {
+  // (HIP launches what is left of 2^32 threads and more along a dimension, without an error)
+  if ((uint64_t)grid.x * threads > 0xffffffffu) return hipErrorInvalidConfiguration;
   std::tuple<P...> args(given...);
   return std::apply(
       [&](P &...p) {
