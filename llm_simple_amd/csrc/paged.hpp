@@ -59,19 +59,22 @@ __device__ __forceinline__ bool token_of(const PagedBatch &p, int b, int token, 
   t = TokenSequence{b, len - end + token};
   return sequence_ok(p, first, end, len) && first <= token && token < end;
 }
-// How many sequences end before or at a token, the same one to all lanes of the wave: the number of the one it belongs to, if no start goes backwards
-__device__ __forceinline__ int ends_upto(const PagedBatch &p, int token, int lane) {
+// How many sequences end before or at a token, the same one to all lanes of the wave: the number of the one it belongs to, if no start goes backwards.
+// ordered: none does of those that were looked at, which are all of them where all end before or at the token.
+__device__ __forceinline__ int ends_upto(const PagedBatch &p, int token, int lane, bool &ordered) {
   int b = 0;
+  ordered = true;
   for (int base = 0; base < p.batch; base += 64) {
-    const int i = base + lane;
-    const bool past = i < p.batch && p.q_starts[min(i, p.batch - 1) + 1] <= token;
+    const int i = base + lane, at = min(i, p.batch - 1), first = p.q_starts[at], end = p.q_starts[at + 1];
+    const bool past = i < p.batch && end <= token;
+    ordered = ordered && __builtin_amdgcn_ballot_w64(first > end) == 0;
     const int count = __builtin_popcountll(__builtin_amdgcn_ballot_w64(past));
     b += count;
     if (count < 64) break;
   }
   return __builtin_amdgcn_readfirstlane(b);
 }
-// The same one to all lanes: looked for in all sequences, as a start that goes backwards asks for, and a token that is none's.  (Always this way:
+// The same one to all lanes: looked for in all sequences, as a start that goes backwards asks for.  (Always this way:
 // append of 8 x 512 tokens of 28 + 2 x 4 heads 18.1 -> 19.0 us, of 300 x 1 5.45 -> 6.6.)
 __device__ __forceinline__ TokenSequence search_sequence(const PagedBatch &p, int token, int lane) {
   for (int base = 0; base < p.batch; base += 64) {
@@ -86,8 +89,10 @@ __device__ __forceinline__ TokenSequence search_sequence(const PagedBatch &p, in
 __device__ __forceinline__ TokenSequence sequence_of(const PagedBatch &p, int token, int lane) {
   TokenSequence t;
   if (p.batch == 1) return token_of(p, 0, token, t) ? t : TokenSequence{-1, -1};
-  const int b = ends_upto(p, token, lane);
+  bool ordered;
+  const int b = ends_upto(p, token, lane, ordered);
   if (__builtin_expect(b < p.batch && token_of(p, b, token, t), 1)) return t;
+  if (b >= p.batch && ordered) return TokenSequence{-1, -1};  // (behind the last one's)
   return search_sequence(p, token, lane);
 }
 
@@ -99,13 +104,15 @@ struct TokenPlace {
 };
 template <int TOKENS> __device__ __forceinline__ TokenPlace token_places(const PagedBatch &p, int token0, int lane) {
   const int token = token0 + min(lane, TOKENS - 1);
-  int b = ends_upto(p, token0, lane);
+  bool ordered;
+  int b = ends_upto(p, token0, lane, ordered);
+  const bool behind = token >= p.tokens || (b >= p.batch && ordered);  // all sequences
   if (token != token0)
     while (b < p.batch && p.q_starts[b + 1] <= token) ++b;
   TokenSequence s = {-1, -1};
   const bool found = b < p.batch && token_of(p, b, token, s);
   if (!found) s = TokenSequence{-1, -1};
-  for (uint64_t left = __builtin_amdgcn_ballot_w64(!found && token < p.tokens); left != 0; left &= left - 1) {
+  for (uint64_t left = __builtin_amdgcn_ballot_w64(!found && !behind); left != 0; left &= left - 1) {
     const int i = __builtin_ctzll(left);
     if (i >= TOKENS) break;
     const TokenSequence x = search_sequence(p, token0 + i, lane);
