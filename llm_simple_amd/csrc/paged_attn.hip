@@ -20,11 +20,15 @@
 // the workgroup that finds all of them stored, tiles' by a second launch, which has the whole chip for them.  A unit of keys is 128 (few rows)
 // or 64.
 //
-// Few rows are bound by the memory system: 16 sequences of 32768 keys of 8 kv heads, 8 bits, 1.08 GB in 170 us, 6.4 TB/s (16 bits 2.15 GB, 326 us,
-// 6.6); a short cache by its chain of memory round trips (starts and lengths, page table, K and V; 384 keys of 2 kv heads 6.5 us, of which an
+// Few rows are bound by the memory system: 16 sequences of 32768 keys of 8 kv heads, 8 bits, 1.08 GB in 171 us, 6.3 TB/s (16 bits 2.15 GB, 326 us,
+// 6.6); a short cache by its chain of memory round trips (starts and lengths, page table, K and V; 384 keys of 2 kv heads 6.4 us, of which an
 // empty launch is 1.6).  Tiles are bound, as the prefill kernels are, by matrix and vector instructions that share a SIMD and the chip's power:
-// a step of two workgroups to a CU takes 2.0-2.2 us, 1.0 PFLOP/s; 4 us of a workgroup's time are its start.  (us: a prompt of 4096 tokens of 28 + 4
-// heads 134, 0.90 PFLOP/s, in 8 bits 131; 200 past 16001 63.5; 8192 with a window of 1024 150.)
+// a step of two workgroups to a CU takes 2.0-2.2 us, 1.0 PFLOP/s; 4 us of a workgroup's time are its start.  (us, on the
+// faster and on the slower of two cards: a prompt of 4096 tokens of 28 + 4 heads 131 / 141, 0.85-0.92 PFLOP/s, in 8 bits 129 / 137; 200 past 16001 60 / 64;
+// 8192 with a window of 1024 147 / 155.  Figures below are pairs of one card each.)
+//
+// More scalars are alive than there are scalar registers, and some are kept in lanes of vector registers: none that a loop over keys asks for, but
+// for the runs in 8 bits, six of the 450 instructions of two steps.
 //
 // Keys that a row must not see: their scores become -inf, so their K does not matter, but a weight of 0 times a V that is not finite
 // would be NaN.  Rows behind the last key, and pages that are not there, are zeros (the loads' descriptors end before them).  V of keys
@@ -386,6 +390,7 @@ struct PagedArguments {  // as the kernels have them
   u32x2_t c;
   PagedAttn p;
 };
+static_assert(__builtin_offsetof(PagedArguments, p) == sizeof(addresses_t) + sizeof(u32x4_t) + sizeof(u32x2_t));
 __device__ __forceinline__ PagedAttn fresh_arguments() {
   typedef __attribute__((address_space(4))) const PagedArguments Constant;
   uint64_t at = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
@@ -1179,9 +1184,9 @@ template <typename T> __device__ __forceinline__ void fold_row(const PagedAttn &
 }
 // Partials of a tile of a kv head, 8 rows to a workgroup, or 16 or 32 one after the other, 32 lanes of 4 dims to a row; 8 partials are on
 // their way at a time.  The more tiles the host counts with, the fewer are split, and a workgroup that finds nothing to fold costs its
-// start (us, 8 rows / 16 / 32, tiles of a kv head by the parts that run at a time: a prompt of 4096, 1.8, 135.5 / 133.3 / 133.2; six of up to 1019
-// of 32 kv heads, 2.7, 71.5 / 70.2 / 67.4; 6 x 700 past 2000, 1.8, 100.8 / 99.1 / 100.6; 4 x 400 past 3000, 0.7, 104.9 / 102.5 / 102; 200 past
-// 16001, 0.1, 64.9 / 67.0 / 69.2).
+// start (us, 8 rows / 16 / 32, tiles of a kv head by the parts that run at a time: a prompt of 4096, 1.8, 143.0 / 141.4 / 140.4; six of up to 1019
+// of 32 kv heads, 2.7, 68.1 / 65.4 / 64.2; six of up to 700 past up to 2000, 1.2, 100.2 / 97.2 / 99.0; 4 x 400 past 3000, 0.7, 97.0 / 94.4 / 93.9;
+// 200 past 16001, 0.1, 65.2 / 65.7 / 67.9; 100 past 4000, 0.05, 22.6 / 23.6 / 27.4).
 template <typename T> __global__ __launch_bounds__(256) void paged_combine_kernel(addresses_t a, u32x4_t b, u32x2_t c_, PagedAttn p) {
   take_early(p, a, b, c_);
   const int tid = threadIdx.x, lane = tid & 63, d4 = (tid & 31) * 4;

@@ -60,9 +60,10 @@ template <typename T> __device__ __forceinline__ void limited8(u32x4_t v, float 
 }
 
 // A workgroup has a token, 8 lanes to a row as in rope_kv_append.hip, 32 rows at a time.  Where the token is is the same to all: scalar
-// work.  Many tokens are bound by the memory system: 4096 of 28 + 2 x 4 heads, 78 MB in and out, in 18.3 us, 4.2 TB/s (a plain copy of as
-// much 16.3); several tokens to a workgroup, and rows dealt to lanes across tokens, were slower (20-23).  Few by their chain of loads, starts to
-// page table to stores: 4.8 us, of which an empty launch is 1.6.
+// work.  Many tokens are bound by the memory system: 4096 of 28 + 2 x 4 heads, 78 MB in and out, in 17.7 us, 4.4 TB/s (a plain copy of as
+// much 16.3; the contiguous cache's kernel, which deals rows to lanes across tokens, 14.4: here 36 rows are two turns of 32, the second with
+// four); in 8 bits, 73 MB, as long.  Several tokens to a workgroup, and rows dealt to lanes across tokens, were slower (20-23).  Few by their chain of
+// loads, starts to page table to stores: 24 in 8 bits 2.8 us, of which an empty launch is 1.6.
 template <typename T, bool NEOX, bool EIGHT> __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppend p) {
   const int token = workgroup(), tid = threadIdx.x, lane = tid & 63, j = tid & 7;
   const TokenSequence s = sequence_of(p.batch, token, lane);
@@ -112,7 +113,7 @@ hipError_t launch_paged_append(void *out_q, void *k_pages, void *v_pages, const 
                                const void *in_k, const void *in_v, int table_rows, int q_heads, int kv_heads, int is_neox, bool eight,
                                int dt, hipStream_t stream) {
   // A token's rows over several workgroups where there are fewer tokens than CUs (us, one / several: 24 tokens of 40 + 2 x 8 heads in 8
-  // bits 5.35 / 4.8; 4096 of 28 + 2 x 4 18.3 / 19.7).
+  // bits 3.4 / 2.8; 300 of 28 + 2 x 4 5.7 / 5.1; 8 x 512 of them 19.1 / 20.8, in 8 bits 19.4 / 21.5).
   const unsigned spread = batch.tokens < device_compute_units() ? (unsigned)(q_heads + 2 * kv_heads + 31) / 32 : 1u;
   const PagedAppend p = {batch,
                          static_cast<char *>(out_q),
@@ -141,7 +142,7 @@ struct PagedRead {
 };
 
 // A workgroup has TOKENS tokens; 16 lanes to a row, 16 rows of a token at a time.  All loads of a turn go out before the first is used.  Bound by
-// the memory system: 32768 rows of 8 kv heads in 8 bits, 202 MB in and out, in 39.7 us, 5.1 TB/s.  (TOKENS, us: 1 56, 2 46, 4 39.7, 8 41; with
+// the memory system: 32768 rows of 8 kv heads in 8 bits, 202 MB in and out, in 39.6 us, 5.1 TB/s.  (TOKENS, us: 1 56, 2 46, 4 39.7, 8 41; with
 // ordinary stores 44.)
 template <typename T, bool EIGHT, int TOKENS> __global__ __launch_bounds__(256) void paged_read_kernel(PagedRead p) {
   const int token0 = workgroup() * TOKENS, tid = threadIdx.x, lane = tid & 63, j = tid & 15;

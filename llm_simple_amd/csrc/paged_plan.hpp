@@ -34,9 +34,9 @@ struct PagedPlan {
 // Wide tiles, 8 waves of 32 rows and one workgroup to a CU, read K and V half as often, and widen 8 bits half as often, but are half as many,
 // to be dealt to half as many places.  They are taken where rows do not fill them much worse than narrow ones, and either long caches
 // behind few tokens, which are cut into parts of about one length, are work for all places, or 8-bit prompts make rounds enough (us, narrow / wide:
-// 500 past 30000 of 28 + 4 heads 235 / 222, in 8 bits 271 / 236; 200 past 16001 65.2 / 63.8, 73.4 / 68.6; 4 x 130 past 9000 88.1 / 84.7; 100 past
-// 4000 22.7 / 26.2; prompts, whose tiles differ in length: of 2048 52.6 / 60, 65 / 66.5, of 4096 139 / 130, 153 / 135, of 6000 268 / 273, 297 / 287,
-// of 4000 of 40 + 8 177 / 183, 197 / 193).
+// 500 past 30000 of 28 + 4 heads 240 / 226, in 8 bits 273 / 239; 200 past 16001 67.2 / 65.5, 73.7 / 69.5; 4 x 130 past 9000 91.0 / 87.6; 100 past
+// 4000 22.6 / 26.3, 27.5 / 30.9; prompts, whose tiles differ in length: of 2048 52.1 / 58.9, 63.4 / 66.4, of 4096 141 / 132, 156 / 137, of 6000 273 / 276,
+// 299 / 291, of 4000 of 40 + 8 180 / 185, 198 / 194).
 inline PagedPlan plan_paged(int tokens, int batch, int max_q_len, int max_kv_len, int window, int sinks, int g, int Hkv, bool eight) {
   PagedPlan pl = {};
   const long long cus = device_compute_units(), sequences = batch < tokens ? batch : tokens;  // that have new tokens at all
